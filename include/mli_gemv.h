@@ -75,7 +75,8 @@ void mli_set_launch_flags(unsigned flags);
  * tensor-core pipeline stalled, 3 a rank's rows of a row-sharded layer never
  * arrived, 4 a chained GEMV's inputs were never completed, 5 the batched
  * tensor-core GEMM met a finite group scale of 2^38 or more (its outputs are
- * not written). */
+ * not written), 6 a page table, sequence number, position or length of a paged
+ * cache pointed outside it (what it pointed at was skipped). */
 int mli_device_error(unsigned* code_out);
 
 /* ---- batch-1 linear ops (the reference's matmul launchers) ------------- */
@@ -377,6 +378,125 @@ int mli_rowshard_wait_argmax(int form, int n, const unsigned long long* logits, 
  * reference's logits copy to the host and host argmax, src/main_cuda.cpp:96-98,
  * src/model_cuda_v2_shared.cu:571-575).  NaN never wins; -0.0 equals +0.0. */
 int mli_argmax(const float* x, int n, long long* out, void* stream);
+
+/* ---- attention over a paged key-value cache ---------------------------- */
+
+/* What a decode step does between its q/k/v and its o projection (the
+ * reference's rope_kernel, KV copies and fused_attention_kernel,
+ * src/model_cuda_v2_shared.cu:233-365 and :388-400), for any number of
+ * sequences whose keys and values live in pages of one cache.  Queries, keys,
+ * values and outputs are fp32, as the linear ops above write and read them. */
+#define MLI_KV_F32 0
+#define MLI_KV_F16 1
+#define MLI_KV_BF16 2
+
+/* A cache: for every layer, `pages` pages of `page_size` slots (one token's
+ * keys or values of all kv_heads heads).  Element e of head h, slot s of page p
+ * of layer l lies at base + l * layer_stride + p * page_stride +
+ * h * head_stride + s * slot_stride + e, strides in elements, the same for k
+ * and v, so pages may be laid out head by head, token by token, or with keys
+ * and values of a page side by side.  k and v 16-byte aligned, strides and
+ * head_dim multiples of 16 bytes, head_dim <= 256 (MLI_ERR_UNSUPPORTED
+ * otherwise); elements must not overlap.  The struct itself is read on the
+ * host during the call. */
+typedef struct mli_kv_cache {
+  void* k;
+  void* v;
+  int dtype; /* MLI_KV_* */
+  int layers, pages, page_size, kv_heads, head_dim;
+  long long layer_stride, page_stride, head_stride, slot_stride;
+} mli_kv_cache;
+
+/* Frequency scalings of mli_rope_turns. */
+#define MLI_ROPE_PLAIN 0  /* theta^(-2i / rot_dim) */
+#define MLI_ROPE_LINEAR 1 /* all of them divided by factor */
+#define MLI_ROPE_LLAMA3 2 /* the reference's get_llama3_scaled_freq (:233-250) */
+#define MLI_ROPE_YARN 3   /* a ramp between the plain and the divided ones */
+
+/* HOST function (no CUDA call): the rotary frequencies of rot_dim / 2 pairs,
+ * in turns (of 2 pi) per position, into the host array `turns`; a caller
+ * copies them to the device once.  `factor` stretches the context; with
+ * LLAMA3 wavelengths above original_len / low are divided by it, those below
+ * original_len / high kept, those between mixed (Llama-3.2: theta 500000,
+ * factor 32, low 1, high 4, original_len 8192); with YARN pairs that turn less than
+ * `low` times over original_len are divided, those that turn more than `high` times
+ * kept (usually 1 and 32). */
+int mli_rope_turns(double* turns, int rot_dim, double theta, int scaling, double factor,
+                   double low, double high, int original_len);
+
+/* m new tokens: per head an optional RMSNorm of q and k
+ * (w * x / sqrt(mean(x^2) + eps) over the head), the rotation of their first
+ * rot_dim values by pos * turns[i] turns, q to q_out, and k and v, rounded to
+ * the cache's type (to nearest even), into their slots of layer `layer`.
+ * Token t is position pos[t] of sequence seq[t] (seq NULL: sequence t); its
+ * page is page_table[seq][pos / page_size], its slot pos % page_size.  A pair
+ * is (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`; both cosine and
+ * sine are multiplied by `amplitude` (1 but for YaRN).  The angle is reduced in
+ * 64 bits, so far positions lose nothing.
+ * A token with pos < 0 is padding: nothing of it is read or written.  One whose
+ * sequence or position lies outside the page table, or whose page lies outside
+ * the cache, gets its q_out, but no slot, and records device error 6.
+ * q_out may be q (same stride); no other buffers may overlap.  Two tokens of one call must not
+ * name the same slot, nor a slot of a page that sequences share. */
+typedef struct mli_rope_op {
+  int m, heads;          /* tokens, query heads (a multiple of the cache's kv_heads) */
+  int rot_dim;           /* even, 0 (no rotation) .. head_dim */
+  int interleaved;
+  float amplitude, eps;
+  const double* turns;   /* [rot_dim / 2] */
+  float* q_out;          /* [m][heads][head_dim], tokens q_out_stride floats apart */
+  const float* q;
+  const float* k;        /* [m][kv_heads][head_dim], tokens k_stride floats apart */
+  const float* v;
+  long long q_out_stride, q_stride, k_stride, v_stride;
+  const float* q_norm;   /* [head_dim], or NULL: no norm */
+  const float* k_norm;
+  const int* pos;        /* [m] */
+  const int* seq;        /* [m], or NULL */
+  const int* page_table; /* [table_rows][table_cols], rows table_stride ints apart */
+  int table_rows, table_cols;
+  long long table_stride;
+} mli_rope_op;
+int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer, void* stream);
+
+/* Attention of one new token a row over its sequence's cached keys and values:
+ * out[r][h] = sum_t p_t v_t, p = softmax over t < lengths[r] of
+ * scale * (q[r][h] . k_t), key-value head h / (heads / kv_heads).  Row r reads
+ * page-table row seq[r] (NULL: row r), so several rows may be tokens of one
+ * sequence (a prompt chunk: lengths pos + 1).  Sums and statistics are fp32,
+ * and q and p enter the products with all their fp32 bits whatever the cache's
+ * type; they and live keys and values are finite (a head with others among them
+ * has outputs that are not).  Slots behind a row's length are not read.  A row of length <= 0 is
+ * zero.  A length beyond the page table is cut to it, keys of a page outside
+ * the cache are left out, and a row whose seq lies outside the table is zero;
+ * each records device error 6.
+ * `workspace`: mli_paged_attention_workspace_bytes bytes of device memory, 16-byte aligned,
+ * zeroed once before its first use; every call leaves it ready for the next,
+ * of any sizes that need no more bytes.  Calls that share a workspace must not overlap on the
+ * GPU.  Results do not change from run to run.  q and out 16-byte aligned, strides multiples of 4 floats. */
+typedef struct mli_attention_op {
+  int rows, heads;
+  float scale;           /* > 0 */
+  float* out;            /* [rows][heads][head_dim], rows out_stride floats apart */
+  const float* q;
+  long long out_stride, q_stride;
+  const int* lengths;    /* [rows] tokens of each row's cache, the new one included */
+  const int* seq;        /* [rows], or NULL */
+  const int* page_table; /* [table_rows][table_cols], rows table_stride ints apart */
+  int table_rows, table_cols;
+  long long table_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} mli_attention_op;
+size_t mli_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
+int mli_paged_attention(const mli_attention_op* op, const mli_kv_cache* cache, int layer, void* stream);
+
+/* Copies page src[i] to page dst[i] for i < n, in every layer, keys and
+ * values: forks of a sequence's last page, moves of a compaction.  Pairs with
+ * a negative src or dst are skipped (padding); pairs outside the cache too, and
+ * they record device error 6.  All copies happen at once: no dst may be
+ * another pair's src or dst. */
+int mli_kv_copy_pages(const mli_kv_cache* cache, const int* src, const int* dst, int n, void* stream);
 
 /* ---- offline weight preparation ---------------------------------------- */
 

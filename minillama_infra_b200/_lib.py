@@ -44,6 +44,36 @@ _OPS = ctypes.POINTER(GemvOp)
 class GemmOp(ctypes.Structure):
     """struct mli_gemm_op (include/mli_gemv.h): one GEMM of a group launch."""
     _fields_ = [("y", _P), ("xq", _P), ("xs", _P), ("w_q", _P), ("w_s", _P), ("n", _I), ("d", _I)]
+
+
+_L = ctypes.c_longlong
+
+
+class KvCacheDesc(ctypes.Structure):
+    """struct mli_kv_cache (include/mli_gemv.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("dtype", _I), ("layers", _I), ("pages", _I), ("page_size", _I),
+                ("kv_heads", _I), ("head_dim", _I), ("layer_stride", _L), ("page_stride", _L),
+                ("head_stride", _L), ("slot_stride", _L)]
+
+
+class RopeOp(ctypes.Structure):
+    """struct mli_rope_op (include/mli_gemv.h)."""
+    _fields_ = [("m", _I), ("heads", _I), ("rot_dim", _I), ("interleaved", _I), ("amplitude", ctypes.c_float),
+                ("eps", ctypes.c_float), ("turns", _P), ("q_out", _P), ("q", _P), ("k", _P), ("v", _P),
+                ("q_out_stride", _L), ("q_stride", _L), ("k_stride", _L), ("v_stride", _L), ("q_norm", _P),
+                ("k_norm", _P), ("pos", _P), ("seq", _P), ("page_table", _P), ("table_rows", _I),
+                ("table_cols", _I), ("table_stride", _L)]
+
+
+class AttentionOp(ctypes.Structure):
+    """struct mli_attention_op (include/mli_gemv.h)."""
+    _fields_ = [("rows", _I), ("heads", _I), ("scale", ctypes.c_float), ("out", _P), ("q", _P),
+                ("out_stride", _L), ("q_stride", _L), ("lengths", _P), ("seq", _P), ("page_table", _P),
+                ("table_rows", _I), ("table_cols", _I), ("table_stride", _L), ("workspace", _P),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+_CACHE = ctypes.POINTER(KvCacheDesc)
 SIGNATURES = {
     "mli_status_string": (ctypes.c_char_p, [_I]),
     "mli_last_status": (_I, []),
@@ -87,6 +117,12 @@ SIGNATURES = {
     "mli_debug_plan_gemm_group": (_I, [ctypes.POINTER(GemmOp), _I, _I, ctypes.POINTER(_I)]),
     "mli_debug_int8_mma_peak": (_I, [_I, _I, _I, _P]),
     "mli_gemm_w8a8_group": (_I, [ctypes.POINTER(GemmOp), _I, _I, _I, _P]),
+    "mli_rope_turns": (_I, [ctypes.POINTER(ctypes.c_double), _I, ctypes.c_double, _I, ctypes.c_double,
+                            ctypes.c_double, ctypes.c_double, _I]),
+    "mli_rope_append": (_I, [ctypes.POINTER(RopeOp), _CACHE, _I, _P]),
+    "mli_paged_attention_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "mli_paged_attention": (_I, [ctypes.POINTER(AttentionOp), _CACHE, _I, _P]),
+    "mli_kv_copy_pages": (_I, [_CACHE, _P, _P, _I, _P]),
 }
 
 # The drop-in shim's C++ symbols (include/mli_gemv.h, reference include/model.h:62-64).

@@ -21,6 +21,7 @@ enum DeviceError : unsigned int {
   kDevPeerTimeout = 3,   // rows of a row-sharded step never arrived from a rank
   kDevChainTimeout = 4,  // a chained GEMV's inputs were never completed
   kDevScaleRange = 5,    // a group scale outside the batched tensor-core path's exact range
+  kDevPageRange = 6,     // a page, sequence, position or length outside a paged cache
 };
 #ifndef MLI_SEPARATE_DEVICE_MODULE
 extern __device__ unsigned int g_device_error;

@@ -1,0 +1,165 @@
+"""Pages of a key-value cache: who holds which, and when one has to be copied.
+
+`PagedKvCache` owns a cache's memory and its page table.  Sequences are rows of
+the page table; a page may belong to several of them (forks), and is copied for
+one of them when that one is about to write into it.  The bookkeeping is on the
+host; the tensors that the kernels read (`cache`, `page_table`) are on the
+device, and every change of them is ordered on the current stream.
+
+    kv = PagedKvCache(layers=16, pages=4096, kv_heads=8, head_dim=64, max_seqs=64)
+    s = kv.new()
+    kv.extend([s], [prompt_len])            # slots for the prompt's tokens
+    ops.rope_append(q, q, k, v, kv.cache, layer, pos, kv.page_table, turns, seq=...)
+    t = kv.fork(s)                          # shares every page
+    kv.extend([s, t])                       # one more token each: t's (or s's) last page is copied
+    kv.free(s); kv.compact()
+"""
+from __future__ import annotations
+
+from . import ops
+
+__all__ = ["PagedKvCache"]
+
+
+class PagedKvCache:
+    """layout "heads" keeps a page's slots of one head together (16-bit heads of
+    64 then make runs of page_size * 128 bytes), "tokens" a token's heads."""
+
+    def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, page_size: int = 16,
+                 max_seqs: int = 64, max_pages: int | None = None, dtype=None, device="cuda",
+                 layout: str = "heads"):
+        import torch
+
+        if layout not in ("heads", "tokens"):
+            raise ValueError("layout: heads or tokens")
+        if min(layers, pages, kv_heads, head_dim, page_size, max_seqs) <= 0:
+            raise ValueError("sizes have to be positive")
+        dtype = torch.bfloat16 if dtype is None else dtype
+        inner = (kv_heads, page_size) if layout == "heads" else (page_size, kv_heads)
+        k, v = (torch.zeros((layers, pages, *inner, head_dim), dtype=dtype, device=device) for _ in range(2))
+        if layout == "tokens":
+            k, v = k.transpose(2, 3), v.transpose(2, 3)
+        self.cache = ops.KvCache(k, v)
+        self.page_size, self.max_pages = page_size, pages if max_pages is None else max_pages
+        # -1 names no page: a kernel that is led there reports it
+        self.page_table = torch.full((max_seqs, self.max_pages), -1, dtype=torch.int32, device=device)
+        self._free_pages = list(range(pages - 1, -1, -1))
+        self._free_rows = list(range(max_seqs - 1, -1, -1))
+        self._holders = [0] * pages
+        self._pages: dict[int, list[int]] = {}
+        self._lengths: dict[int, int] = {}
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free_pages)
+
+    def length(self, seq: int) -> int:
+        return self._lengths[seq]
+
+    def pages(self, seq: int) -> list[int]:
+        return list(self._pages[seq])
+
+    def new(self) -> int:
+        """An empty sequence: its row of the page table."""
+        if not self._free_rows:
+            raise MemoryError("every row of the page table is in use")
+        seq = self._free_rows.pop()
+        self._pages[seq], self._lengths[seq] = [], 0
+        return seq
+
+    def extend(self, seqs, counts=None) -> None:
+        """Slots for counts[i] (one) more tokens of seqs[i].  All or nothing: without
+        pages enough, MemoryError, and nothing has changed."""
+        seqs = list(seqs)
+        counts = [1] * len(seqs) if counts is None else list(counts)
+        if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(n < 0 for n in counts):
+            raise ValueError("expected distinct sequences and a count >= 0 for each")
+        # how many hold each page, as the copies below change it
+        holders = {p: self._holders[p] for s in seqs for p in self._pages[s][-1:]}
+        copies, needed = [], 0
+        for seq, n in zip(seqs, counts):
+            have, length = self._pages[seq], self._lengths[seq]
+            want = -(-(length + n) // self.page_size)
+            if want > self.max_pages:
+                raise MemoryError(f"sequence {seq}: {length + n} tokens need more than {self.max_pages} pages")
+            needed += want - len(have)
+            if n and length % self.page_size and holders[have[-1]] > 1:
+                holders[have[-1]] -= 1
+                copies.append(seq)
+                needed += 1
+        if needed > len(self._free_pages):
+            raise MemoryError(f"{needed} pages needed, {len(self._free_pages)} free")
+        moved = []
+        for seq in copies:
+            old, page = self._pages[seq][-1], self._take()
+            self._holders[old] -= 1
+            self._pages[seq][-1] = page
+            moved.append((old, page))
+        changed = set(copies)
+        for seq, n in zip(seqs, counts):
+            self._lengths[seq] += n
+            while len(self._pages[seq]) * self.page_size < self._lengths[seq]:
+                self._pages[seq].append(self._take())
+                changed.add(seq)
+        self._copy(moved)
+        self._upload(changed)
+
+    def fork(self, seq: int) -> int:
+        """A new sequence that starts with all of seq's tokens and shares its pages."""
+        new = self.new()
+        self._pages[new], self._lengths[new] = list(self._pages[seq]), self._lengths[seq]
+        for page in self._pages[new]:
+            self._holders[page] += 1
+        self._upload([new])
+        return new
+
+    def free(self, seq: int) -> None:
+        """Gives the sequence's row back, and the pages that no other holds."""
+        for page in self._pages.pop(seq):
+            self._holders[page] -= 1
+            if not self._holders[page]:
+                self._free_pages.append(page)
+        del self._lengths[seq]
+        self._free_rows.append(seq)
+        self.page_table[seq].fill_(-1)
+
+    def compact(self) -> int:
+        """Moves pages so that those in use are the first ones; how many moved."""
+        used = sum(1 for n in self._holders if n)
+        holes = [p for p in range(used) if not self._holders[p]]
+        # each move goes from behind `used` to before it: no page is both source and destination
+        moved = dict(zip((p for p in range(used, len(self._holders)) if self._holders[p]), holes))
+        if not moved:
+            return 0
+        self._copy(list(moved.items()))
+        for old, page in moved.items():
+            self._holders[page], self._holders[old] = self._holders[old], 0
+        changed = []
+        for seq, pages in self._pages.items():
+            if any(p in moved for p in pages):
+                self._pages[seq] = [moved.get(p, p) for p in pages]
+                changed.append(seq)
+        self._free_pages = list(range(len(self._holders) - 1, used - 1, -1))
+        self._upload(changed)
+        return len(moved)
+
+    def _take(self) -> int:
+        page = self._free_pages.pop()
+        self._holders[page] = 1
+        return page
+
+    def _copy(self, pairs) -> None:
+        import torch
+
+        if pairs:
+            both = torch.tensor(pairs, dtype=torch.int32, device=self.page_table.device).T.contiguous()
+            ops.kv_copy_pages(self.cache, both[0], both[1])
+
+    def _upload(self, seqs) -> None:
+        import torch
+
+        for seq in seqs:
+            pages = self._pages[seq]
+            if pages:
+                self.page_table[seq, :len(pages)] = torch.tensor(pages, dtype=torch.int32,
+                                                                 device=self.page_table.device)

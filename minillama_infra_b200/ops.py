@@ -16,13 +16,14 @@ from __future__ import annotations
 
 import ctypes
 
-from ._lib import GemvOp, check, lib
+from ._lib import AttentionOp, GemvOp, KvCacheDesc, RopeOp, check, lib
 
 __all__ = [
     "matmul", "matmul_int8", "matmul_dp4a", "quantize_activation", "matmul_dp4a_fused",
     "quantize_activation_rows", "gemm_w8a8", "gemm_w8a8_cuda_core", "gemm_workspace_bytes",
     "quantize_weights", "group_dots",
     "device_error", "set_pdl", "copy_from_ptr", "GemvChain", "DECODE_LAYER_WAITS",
+    "KvCache", "rope_turns", "rope_append", "paged_attention", "paged_attention_workspace", "kv_copy_pages",
 ]
 
 
@@ -296,3 +297,172 @@ class GemvChain:
             self.close()
         except Exception:
             pass
+
+
+# ---- attention over a paged key-value cache ---------------------------------
+_KV_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+_ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
+
+
+class KvCache:
+    """A paged key-value cache as the kernels see it (struct mli_kv_cache).
+
+    k, v: tensors [layers, pages, kv_heads, page_size, head_dim] of one type
+    (fp32, fp16 or bf16) with the same strides, the last dimension contiguous:
+    pages laid out token by token are given as `t.transpose(2, 3)`, keys and
+    values that share pages as two views of one tensor.  The tensors stay the
+    caller's; the handle keeps references to them.
+    """
+
+    def __init__(self, k, v):
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("expected k and v of one shape [layers, pages, kv_heads, page_size, head_dim], "
+                             "one type and one device")
+        if str(k.dtype) not in _KV_DTYPES:
+            raise ValueError(f"a cache is fp32, fp16 or bf16, not {k.dtype}")
+        # the stride of a dimension of one entry is never used
+        strides = [0 if n == 1 else s for n, s in zip(k.shape, k.stride())]
+        if strides != [0 if n == 1 else s for n, s in zip(v.shape, v.stride())] or strides[4] > 1:
+            raise ValueError("expected k and v of the same strides, the last dimension contiguous")
+        self.k, self.v = k, v
+        self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = k.get_device()  # -1: host memory, which no kernel takes
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _KV_DTYPES[str(k.dtype)], self.layers, self.pages,
+                                self.page_size, self.kv_heads, self.head_dim, *strides[:4])
+        self.ref = ctypes.byref(self.desc)
+
+
+def _on_device(device: int, stream, call, what: str) -> None:
+    """call(stream) with `device` current, on `stream` or that device's current one."""
+    import torch
+
+    if device < 0:
+        raise ValueError("expected a CUDA tensor (device memory)")
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if torch.cuda.current_device() == device:
+        check(call(handle), what)
+    else:
+        with torch.cuda.device(device):
+            check(call(handle), what)
+
+
+def _head_rows(t, name, rows, heads, dim, device):
+    """(pointer, floats between rows) of an fp32 tensor [rows, heads, dim] whose rows are contiguous."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or (rows is not None and shape[0] != rows) or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name}: expected [{'rows' if rows is None else rows}, {heads}, {dim}], got {list(shape)}")
+    if str(t.dtype) != "torch.float32" or t.get_device() != device:
+        raise ValueError(f"{name}: expected an fp32 tensor on the cache's device")
+    if (dim > 1 and strides[2] != 1) or (heads > 1 and strides[1] != dim):
+        raise ValueError(f"{name}: expected contiguous heads within a row")
+    return t.data_ptr(), strides[0] if shape[0] > 1 else heads * dim
+
+
+def _vector(t, name, n, dtype, device):
+    """Pointer of a contiguous 1-D tensor of n entries (None: no pointer)."""
+    if t is None:
+        return None
+    if t.dim() != 1 or t.numel() != n or str(t.dtype) != dtype or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {n} entries on the cache's device")
+    return t.data_ptr()
+
+
+def _table(t, device):
+    """(pointer, rows, columns, ints between rows) of a page table [sequences, pages]."""
+    if t.dim() != 2 or str(t.dtype) != "torch.int32" or t.get_device() != device:
+        raise ValueError("page_table: expected an int32 tensor [sequences, pages] on the cache's device")
+    (rows, cols), strides = t.shape, t.stride()
+    if cols > 1 and strides[1] != 1:
+        raise ValueError("page_table: expected contiguous rows")
+    return t.data_ptr(), rows, cols, strides[0] if rows > 1 else cols
+
+
+def rope_turns(rot_dim: int, theta: float = 500000.0, scaling: str = "none", factor: float = 1.0,
+               low: float = 1.0, high: float = 4.0, original_len: int = 8192, device="cuda"):
+    """Rotary frequencies of rot_dim / 2 pairs in turns per position, a float64
+    tensor on `device` for rope_append (mli_rope_turns).  Llama-3.2:
+    scaling="llama3", factor=32.  "yarn" takes low=1, high=32, and
+    rope_append an amplitude of 0.1 ln(factor) + 1."""
+    import torch
+
+    if scaling not in _ROPE_SCALINGS:
+        raise ValueError(f"scaling: one of {sorted(_ROPE_SCALINGS)}, not {scaling!r}")
+    out = (ctypes.c_double * max(1, rot_dim // 2))()
+    check(lib().mli_rope_turns(out, rot_dim, theta, _ROPE_SCALINGS[scaling], factor, low, high, original_len),
+          "rope_turns")
+    return torch.tensor(list(out), dtype=torch.float64, device=device)
+
+
+def rope_append(q_out, q, k, v, cache: KvCache, layer: int, pos, page_table, turns, seq=None,
+                interleaved: bool = False, amplitude: float = 1.0, q_norm=None, k_norm=None, eps: float = 1e-5,
+                stream=None):
+    """Norms of queries and keys (optional), rotary positions, and the append of
+    keys and values to layer `layer` of a paged cache, in one launch
+    (mli_rope_append; the reference's rope_kernel and KV copies, :233-281 and
+    :391-392).
+
+    q [m, heads, dim], k, v [m, kv_heads, dim]: fp32, rows may be strided (slices
+    of one fused projection).  q_out like q, and may be q.  pos int32 [m]
+    (negative: padding, skipped); seq int32 [m], the token's row of page_table
+    (None: its own number).  turns: rope_turns (None: no rotation).
+    """
+    d, device = cache.head_dim, cache.device
+    m, heads = q.shape[0], q.shape[1]
+    q_ptr, q_stride = _head_rows(q, "q", None, heads, d, device)
+    o_ptr, o_stride = _head_rows(q_out, "q_out", m, heads, d, device)
+    k_ptr, k_stride = _head_rows(k, "k", m, cache.kv_heads, d, device)
+    v_ptr, v_stride = _head_rows(v, "v", m, cache.kv_heads, d, device)
+    t_ptr, t_rows, t_cols, t_stride = _table(page_table, device)
+    pairs = 0 if turns is None else turns.numel()
+    op = RopeOp(m, heads, 2 * pairs, int(interleaved), amplitude, eps,
+                _vector(turns, "turns", pairs, "torch.float64", device), o_ptr, q_ptr, k_ptr, v_ptr, o_stride,
+                q_stride, k_stride, v_stride, _vector(q_norm, "q_norm", d, "torch.float32", device),
+                _vector(k_norm, "k_norm", d, "torch.float32", device),
+                _vector(pos, "pos", m, "torch.int32", device), _vector(seq, "seq", m, "torch.int32", device),
+                t_ptr, t_rows, t_cols, t_stride)
+    _on_device(device, stream, lambda s: lib().mli_rope_append(op, cache.ref, layer, s), "rope_append")
+
+
+def paged_attention_workspace(cache: KvCache, rows: int, heads: int):
+    """A zeroed workspace for paged_attention calls of up to `rows` rows."""
+    import torch
+
+    n = int(lib().mli_paged_attention_workspace_bytes(rows, heads, cache.kv_heads, cache.head_dim))
+    if n == 0:
+        raise ValueError("rows and heads: positive, heads a multiple of the cache's")
+    return torch.zeros(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attention(out, q, cache: KvCache, layer: int, page_table, lengths, scale: float, workspace, seq=None,
+                    stream=None):
+    """Attention of one new token a row over layer `layer` of a paged cache
+    (mli_paged_attention; the reference's fused_attention_kernel, :291-365).
+
+    q, out [rows, heads, dim] fp32; lengths int32 [rows], tokens of each row's
+    cache, the new one included (<= 0: the row is zero); seq int32 [rows], the
+    row's row of page_table (None: its own number).  workspace:
+    paged_attention_workspace; calls that share one must not overlap.
+    """
+    d, device = cache.head_dim, cache.device
+    rows, heads = q.shape[0], q.shape[1]
+    q_ptr, q_stride = _head_rows(q, "q", None, heads, d, device)
+    o_ptr, o_stride = _head_rows(out, "out", rows, heads, d, device)
+    t_ptr, t_rows, t_cols, t_stride = _table(page_table, device)
+    op = AttentionOp(rows, heads, scale, o_ptr, q_ptr, o_stride, q_stride,
+                     _vector(lengths, "lengths", rows, "torch.int32", device),
+                     _vector(seq, "seq", rows, "torch.int32", device), t_ptr, t_rows, t_cols, t_stride,
+                     _vector(workspace, "workspace", workspace.numel(), "torch.uint8", device), workspace.numel())
+    _on_device(device, stream, lambda s: lib().mli_paged_attention(op, cache.ref, layer, s), "paged_attention")
+
+
+def kv_copy_pages(cache: KvCache, src, dst, stream=None):
+    """Copies pages src[i] to dst[i] (int32 tensors) in every layer of a cache,
+    keys and values; pairs with a negative entry are skipped.  No dst may be
+    another pair's src or dst."""
+    n = src.numel()
+    s_ptr = _vector(src, "src", n, "torch.int32", cache.device)
+    d_ptr = _vector(dst, "dst", n, "torch.int32", cache.device)
+    _on_device(cache.device, stream, lambda s: lib().mli_kv_copy_pages(cache.ref, s_ptr, d_ptr, n, s),
+               "kv_copy_pages")
