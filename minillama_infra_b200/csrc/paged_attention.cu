@@ -18,9 +18,10 @@
 // finish where a segment spans several, in CTA order: results do not depend on
 // timing.
 //
-// Each warp streams its tiles through a ring of its own in shared memory
-// (16-byte cp.async, chunks of a row permuted by its number so that column reads
-// do not collide); warps never wait for one another before the join.
+// Each warp streams its tiles through a ring of its own in shared memory, a
+// slot for a tile's keys, the next for its values (16-byte cp.async, chunks of a
+// row permuted by its number so that column reads do not collide); warps never
+// wait for one another before the join.
 #include <float.h>
 #include <math.h>
 
@@ -31,11 +32,10 @@
 namespace mli {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kGroup = 8;          // query heads that share a pass over a segment
-constexpr int kStageBytes = 16384;  // one tile of keys and of values
-constexpr int kMaxCtas = 160;       // CTAs with partial results in the workspace
+constexpr int kGroup = 8;         // query heads that share a pass over a segment
+constexpr int kSlotBytes = 8192;  // one tile's keys, or its values
+constexpr int kSlots = 3;         // of a warp's ring
+constexpr int kMaxCtas = 160;     // CTAs with partial results in the workspace
 
 // ---- division of n < 2^31 by a number known at launch ------------------------
 struct FastDiv {
@@ -51,15 +51,22 @@ __device__ __forceinline__ unsigned divide(unsigned n, const FastDiv& d) {
   return static_cast<unsigned>((static_cast<unsigned long long>(n) * d.mul) >> d.shift);
 }
 
-__device__ __forceinline__ void cp_async16(void* smem, const void* src, bool live) {
-  // a chunk that is not live is filled with zeros, its source not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(src), "r"(live ? 16 : 0)
-               : "memory");
+__device__ __forceinline__ void cp_async16(unsigned smem, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
+}
+// The same where `live`, else zeros, the source not read.
+__device__ __forceinline__ void cp_async16(unsigned smem, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 struct Args {
@@ -76,19 +83,19 @@ struct Args {
   int chunks;      // passes of up to kGroup of them
   float scale;     // times log2(e)
   FastDiv page_div;
-  float* partials;     // [kMaxCtas][2] pieces
+  void* partials;      // [kMaxCtas][2] pieces
   unsigned* arrivals;  // [rows * kv_heads * chunks], zero between calls
 };
 
 // A piece of a segment: the unnormalised output, the maximum, the sum and c of each head.
-template <int kDim>
+template <int kDim, int kHeads>
 struct Piece {
-  float o[kGroup][kDim];
-  float m[kGroup], l[kGroup], c[kGroup];
+  float o[kHeads][kDim];
+  float m[kHeads], l[kHeads], c[kHeads], pad[kHeads];
 };
 // What a piece of maximum m counts beside one of maximum top (no piece: 1, and its sums are zero).
 __device__ __forceinline__ float piece_weight(float m, float top, float c) {
-  return m == top ? 1.f : exp2f((m - top) * c);
+  return m == top ? 1.f : exp2_approx((m - top) * c);
 }
 
 // ---- the products on the tensor cores, 16-bit caches --------------------------
@@ -111,13 +118,6 @@ struct Pair<__nv_bfloat16> {
   static __device__ __forceinline__ float2 unpack(unsigned u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
-                                             unsigned b0, unsigned b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
 };
 template <>
 struct Pair<__half> {
@@ -128,14 +128,23 @@ struct Pair<__half> {
   static __device__ __forceinline__ float2 unpack(unsigned u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
-                                             unsigned b0, unsigned b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
 };
+// d = a b, or d += a b
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                    unsigned b1, bool fresh) {
+  const float c[4] = {fresh ? 0.f : d[0], fresh ? 0.f : d[1], fresh ? 0.f : d[2], fresh ? 0.f : d[3]};
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 
 // The three 16-bit parts of two floats.
 template <typename T>
@@ -161,17 +170,25 @@ __device__ __forceinline__ void ldmatrix4_trans(unsigned (&r)[4], unsigned addr)
                : "r"(addr)
                : "memory");
 }
+// Shared address of chunk `chunk ^ row & 7` given that of chunk `x` of the same row, x < 8 (rows begin on 128 bytes).
+__device__ __forceinline__ unsigned swizzled(unsigned first, int chunk) {
+  return (first ^ ((chunk & 7) << 4)) + ((chunk >> 3) << 7);
+}
 
 // kDim: the head dimension's room in shared memory (64, 128 or 256).  kFew: at most 4 heads.
 template <typename T, int kDim, bool kFew>
 struct TensorMath {
-  static constexpr int kTok = kStageBytes / (2 * kDim * 2);  // 64, 32 or 16 tokens a tile
+  static constexpr int kTok = kSlotBytes / (kDim * 2);  // 64, 32 or 16 tokens a tile
+  static constexpr int kHeads = kFew ? 4 : 8;
+  static constexpr int kScratch = 0;
   static constexpr int kSteps = kDim / 16;
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;
+  using Part = Piece<kDim, kHeads>;
 
   unsigned q[kSteps][kFew ? 4 : 6];
-  float o[kDim / 8][2];
-  float m, l, c;
+  unsigned p[kTok / 8][kFew ? 2 : 3];
+  float2 o[kDim / 8];
+  float m, l, c, keep;
   int head;  // this lane's head within the pass
   bool third;
 
@@ -214,36 +231,31 @@ struct TensorMath {
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i) o[i][0] = o[i][1] = 0.f;
+    for (int i = 0; i < kDim / 8; ++i) o[i] = make_float2(0.f, 0.f);
   }
 
-  // live: bit t for token t of the tile
-  __device__ __forceinline__ void tile(const unsigned char* slot, unsigned long long live, float*) {
-    const int lane = threadIdx.x & 31;
-    const unsigned keys = smem_u32(slot), values = keys + kTok * kDim * 2;
-    const int mat = lane >> 3, in = lane & 7;
+  // The tile's weights from its keys.  live: bit t for token t.
+  __device__ __forceinline__ void scores(unsigned keys, unsigned long long live, float*) {
+    const int lane = threadIdx.x & 31, mat = lane >> 3, in = lane & 7;
     float s[kTok / 8][4];
+    // matrices (tokens 0-7, 8-15) x (dims 0-7, 8-15) of a 16-token block
+    const unsigned row = keys + ((mat >> 1) * 8 + in) * (kDim * 2) + (((mat & 1) ^ in) << 4);
 #pragma unroll
-    for (int n = 0; n < kTok / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    {
-      // matrices (tokens 0-7, 8-15) x (dims 0-7, 8-15) of a 16-token block
-      const unsigned row = keys + ((mat >> 1) * 8 + in) * (kDim * 2);
+    for (int k = 0; k < kSteps; ++k) {
+      const unsigned at = swizzled(row, 2 * k);
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const unsigned chunk = ((2 * k + (mat & 1)) ^ in) * 16;
+      for (int n = 0; n < kTok / 16; ++n) {
+        unsigned b[4];
+        ldmatrix4(b, at + n * 16 * (kDim * 2));
 #pragma unroll
-        for (int n = 0; n < kTok / 16; ++n) {
-          unsigned b[4];
-          ldmatrix4(b, row + n * 16 * (kDim * 2) + chunk);
-          Pair<T>::mma(s[2 * n], q[k][0], q[k][1], q[k][2], q[k][3], b[0], b[1]);
-          Pair<T>::mma(s[2 * n + 1], q[k][0], q[k][1], q[k][2], q[k][3], b[2], b[3]);
-          if (!kFew) {
-            Pair<T>::mma(s[2 * n], q[k][4], 0u, q[k][5], 0u, b[0], b[1]);
-            Pair<T>::mma(s[2 * n + 1], q[k][4], 0u, q[k][5], 0u, b[2], b[3]);
-          }
+        for (int h = 0; h < 2; ++h) {
+          float(&d)[4] = s[2 * n + h];
+          mma<T>(d, q[k][0], q[k][1], q[k][2], q[k][3], b[2 * h], b[2 * h + 1], k == 0);
+          if (!kFew) mma<T>(d, q[k][4], 0u, q[k][5], 0u, b[2 * h], b[2 * h + 1], false);
         }
       }
     }
+    constexpr unsigned long long kAll = ~0ull >> (64 - kTok);
     float top = m;
 #pragma unroll
     for (int n = 0; n < kTok / 8; ++n)
@@ -251,46 +263,60 @@ struct TensorMath {
       for (int j = 0; j < 2; ++j) {
         float x = s[n][j] + s[n][j + 2];
         if (kFew) x += __shfl_xor_sync(0xffffffffu, x, 16);
-        x = (live >> (8 * n + 2 * (lane & 3) + j)) & 1 ? x : -INFINITY;
         s[n][j] = x;
-        top = fmaxf(top, x);
       }
+    if (live != kAll) {
+      const unsigned long long mine = live >> (2 * (lane & 3));
+#pragma unroll
+      for (int n = 0; n < kTok / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[n][j] = (mine >> (8 * n + j)) & 1 ? s[n][j] : -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < kTok / 8; ++n) top = fmaxf(top, fmaxf(s[n][0], s[n][1]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float base = top == -INFINITY ? 0.f : top;
-    const float keep = exp2f((m - base) * c);  // m = -inf: 0
+    keep = exp2_approx((m - base) * c);  // m = -inf: 0
     m = top;
     l *= keep;
-    unsigned p[kTok / 8][3];
 #pragma unroll
     for (int n = 0; n < kTok / 8; ++n) {
-      const float x = exp2f((s[n][0] - base) * c), y = exp2f((s[n][1] - base) * c);
+      const float x = exp2_approx((s[n][0] - base) * c), y = exp2_approx((s[n][1] - base) * c);
       l += x + y;
       unsigned hi, mid, lo;
       split3<T>(x * kUp, y * kUp, hi, mid, lo);
       p[n][0] = third ? 0u : hi;
       p[n][1] = third ? lo : mid;
-      p[n][2] = lo;
+      if (!kFew) p[n][2] = lo;
     }
-    const unsigned row = values + ((mat & 1) * 8 + in) * (kDim * 2);
+  }
+
+  // The tile's outputs from its values.  A tile's sum starts from zero, so that the tensor cores' accumulation
+  // (which truncates) never runs over more than a tile.
+  __device__ __forceinline__ void outputs(unsigned values, float*) {
+    const int lane = threadIdx.x & 31, mat = lane >> 3, in = lane & 7;
+    const unsigned row = values + ((mat & 1) * 8 + in) * (kDim * 2) + (((mat >> 1) ^ in) << 4);
+    const float2 keep2 = make_float2(keep, keep);
 #pragma unroll
     for (int d = 0; d < kDim / 16; ++d) {
-      float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      const unsigned chunk = ((2 * d + (mat >> 1)) ^ in) * 16;
+      float acc[2][4];
+      const unsigned at = swizzled(row, 2 * d);
 #pragma unroll
       for (int n = 0; n < kTok / 16; ++n) {
         unsigned b[4];
-        ldmatrix4_trans(b, row + n * 16 * (kDim * 2) + chunk);
+        ldmatrix4_trans(b, at + n * 16 * (kDim * 2));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          Pair<T>::mma(acc[h], p[2 * n][0], p[2 * n][1], p[2 * n + 1][0], p[2 * n + 1][1], b[2 * h], b[2 * h + 1]);
-          if (!kFew) Pair<T>::mma(acc[h], p[2 * n][2], 0u, p[2 * n + 1][2], 0u, b[2 * h], b[2 * h + 1]);
+          mma<T>(acc[h], p[2 * n][0], p[2 * n][1], p[2 * n + 1][0], p[2 * n + 1][1], b[2 * h], b[2 * h + 1],
+                 n == 0);
+          if (!kFew) mma<T>(acc[h], p[2 * n][2], 0u, p[2 * n + 1][2], 0u, b[2 * h], b[2 * h + 1], false);
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) o[2 * d + h][j] = fmaf(o[2 * d + h][j], keep, acc[h][j] + acc[h][j + 2]);
+        o[2 * d + h] = fma2(o[2 * d + h], keep2,
+                            add2(make_float2(acc[h][0], acc[h][1]), make_float2(acc[h][2], acc[h][3])));
     }
   }
 
@@ -301,8 +327,8 @@ struct TensorMath {
     if (kFew) {
 #pragma unroll
       for (int i = 0; i < kDim / 8; ++i) {
-        o[i][0] += __shfl_xor_sync(0xffffffffu, o[i][0], 16);
-        o[i][1] += __shfl_xor_sync(0xffffffffu, o[i][1], 16);
+        o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, 16);
+        o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, 16);
       }
     }
   }
@@ -313,15 +339,14 @@ struct TensorMath {
     float* row = out + head * dim + 2 * (threadIdx.x & 3);
 #pragma unroll
     for (int i = 0; i < kDim / 8; ++i)
-      if (8 * i < dim) *reinterpret_cast<float2*>(row + 8 * i) = make_float2(o[i][0] * inv, o[i][1] * inv);
+      if (8 * i < dim) *reinterpret_cast<float2*>(row + 8 * i) = make_float2(o[i].x * inv, o[i].y * inv);
   }
-  __device__ __forceinline__ void store(Piece<kDim>& to) {
+  __device__ __forceinline__ void store(Part& to) {
     finish();
     if (third) return;
     const int col = 2 * (threadIdx.x & 3);
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i)
-      *reinterpret_cast<float2*>(&to.o[head][8 * i + col]) = make_float2(o[i][0], o[i][1]);
+    for (int i = 0; i < kDim / 8; ++i) *reinterpret_cast<float2*>(&to.o[head][8 * i + col]) = o[i];
     if (col == 0) {
       to.m[head] = m;
       to.l[head] = l * kUp;
@@ -335,17 +360,24 @@ struct TensorMath {
 // A lane takes one token of the tile (or a part of its dims) for the scores
 // and four dims of a token (or eight) for the outputs; q and p come from shared memory
 // as broadcasts.
+__device__ __forceinline__ const float4* shared_float4(unsigned addr) {
+  return reinterpret_cast<const float4*>(__cvta_shared_to_generic(addr));
+}
+
 template <int kDim, bool kFew>
 struct FloatMath {
-  static constexpr int kTok = kStageBytes / (2 * kDim * 4);  // 32, 16 or 8 tokens a tile
+  static constexpr int kTok = kSlotBytes / (kDim * 4);  // 32, 16 or 8 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
+  static constexpr int kScratch = kHeads * (kDim + kTok);  // floats: q, then the tile's p
   static constexpr int kParts = 32 / kTok;   // lanes of a token's score
   static constexpr int kChunks = kDim / 4;   // 16-byte pieces of a token
   static constexpr int kRows = kChunks < 32 ? 32 / kChunks : 1;  // tokens side by side in the outputs' sum
   static constexpr int kOwn = kChunks < 32 ? 1 : kChunks / 32;   // pieces of a token a lane sums
 
+  using Part = Piece<kDim, kHeads>;
+
   float2 o[kHeads][kOwn][2];
-  float m[kHeads], l[kHeads], c;
+  float m[kHeads], l[kHeads], keep[kHeads], c;
 
   __device__ __forceinline__ void begin(const Args& a, const float* qp, int heads, int dim, float* scratch) {
     const int lane = threadIdx.x & 31;
@@ -367,10 +399,9 @@ struct FloatMath {
     }
   }
 
-  __device__ __forceinline__ void tile(const unsigned char* slot, unsigned long long live, float* scratch) {
+  __device__ __forceinline__ void scores(unsigned slot, unsigned long long live, float* scratch) {
     const int lane = threadIdx.x & 31;
-    const float4* keys = reinterpret_cast<const float4*>(slot);
-    const float4* values = keys + kTok * kChunks;
+    const float4* keys = shared_float4(slot);
     const float4* qs = reinterpret_cast<const float4*>(scratch);
     float* ps = scratch + kHeads * kDim;  // [kTok][kHeads]
     const int t = lane % kTok, part = lane / kTok;
@@ -387,7 +418,6 @@ struct FloatMath {
         acc[h][1] = fma2(make_float2(x.z, x.w), make_float2(y.z, y.w), acc[h][1]);
       }
     }
-    float keep[kHeads];
     const bool on = (live >> t) & 1;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
@@ -400,13 +430,19 @@ struct FloatMath {
       for (int off = kTok / 2; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       top = fmaxf(top, m[h]);
       const float base = top == -INFINITY ? 0.f : top;
-      keep[h] = exp2f((m[h] - base) * c);
+      keep[h] = exp2_approx((m[h] - base) * c);
       m[h] = top;
-      const float p = exp2f((s - base) * c);
+      const float p = exp2_approx((s - base) * c);
       l[h] = fmaf(l[h], keep[h], part == 0 ? p : 0.f);
       if (part == 0) ps[t * kHeads + h] = p;
     }
     __syncwarp();
+  }
+
+  __device__ __forceinline__ void outputs(unsigned slot, float* scratch) {
+    const int lane = threadIdx.x & 31;
+    const float4* values = shared_float4(slot);
+    const float* ps = scratch + kHeads * kDim;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h)
 #pragma unroll
@@ -466,7 +502,7 @@ struct FloatMath {
       }
     }
   }
-  __device__ __forceinline__ void store(Piece<kDim>& to) {
+  __device__ __forceinline__ void store(Part& to) {
     finish();
     const int lane = threadIdx.x & 31;
     if (kRows > 1 && lane >= kChunks) return;
@@ -508,64 +544,50 @@ struct Segment {
   int tiles, tokens;
 };
 
-// A warp's walk over the tiles [at, end).
-template <int kTok>
-struct Walk {
-  Segment s;
-  long long at, end;
-
-  __device__ __forceinline__ void advance(const Args& a, int items) {
-    if (++at < s.start + s.tiles || at >= end) return;
-    s.start += s.tiles;
-    if (++s.item < items) return;
-    s.item = 0;
-    bool bad;
-    do {
-      s.tokens = row_tokens(a, ++s.row, &bad);
-    } while (s.tokens == 0 && s.row + 1 < a.rows);
-    s.tiles = (s.tokens + kTok - 1) / kTok;
-  }
-};
-
-enum : int { kFirst = 1, kLast = 2, kWhole = 4 };  // a tile's place in its piece; the piece is a whole segment
-
-struct TileInfo {
-  unsigned long long live;
-  long long start;  // the segment's first tile
-  int row, item, tiles, flags;
-};
-
-// What a CTA knows of a piece it holds in shared memory.
+// A piece that a CTA holds in shared memory.
 struct Held {
   long long start;  // the segment's first tile
   int row, item, tiles, used;
 };
 
-template <typename Math, typename T, int kDim, int kStages>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args a, const CacheLayer<T> cache) {
-  constexpr int kTok = Math::kTok;
-  constexpr int kChunks = kDim * sizeof(T) / 16;  // 16-byte pieces of a token's keys
-  constexpr int kPer = kTok > 32 ? kTok / 32 : 1;  // tokens whose place a lane looks up
-  constexpr bool kFloat = sizeof(T) == 4;
-  constexpr int kScratch = kFloat ? kGroup * kDim + kTok * kGroup : 0;  // floats of FloatMath's q and p
+// Bytes of a warp, and how many of them an SM's 227 KB hold beside the static arrays and 128 bytes for alignment.
+constexpr int kSmemRoom = 232448 - 1024 - 128;
+template <typename Math>
+constexpr int kWarpBytes = kSlots * kSlotBytes + sizeof(typename Math::Part) + Math::kScratch * 4;
+template <typename Math>
+constexpr int kWarpsOf = kSmemRoom / kWarpBytes<Math> < 8 ? kSmemRoom / kWarpBytes<Math> : 8;
 
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_scan[kThreads / 32];
+template <typename Math, typename T, int kDim>
+__global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel(const Args a,
+                                                                                 const CacheLayer<T> cache) {
+  using Part = typename Math::Part;
+  constexpr int kWarps = kWarpsOf<Math>, kThreads = kWarps * 32;
+  constexpr int kTok = Math::kTok;
+  constexpr int kRowBytes = kDim * sizeof(T);
+  constexpr int kChunks = kRowBytes / 16;          // 16-byte pieces of a token's keys
+  constexpr int kPer = kTok > 32 ? kTok / 32 : 1;  // tokens whose place a lane looks up
+  constexpr unsigned long long kAll = ~0ull >> (64 - kTok);
+
+  extern __shared__ unsigned char smem_any[];
+  __shared__ long long s_scan[kWarps];
   __shared__ Segment s_first[kWarps];
-  __shared__ TileInfo s_info[kWarps][kStages];
   __shared__ Held s_held[2 * kWarps];
   __shared__ int s_last;
-  // rings, then two pieces of each warp, then FloatMath's scratch
-  Piece<kDim>* pieces = reinterpret_cast<Piece<kDim>*>(smem + kWarps * kStages * kStageBytes);
-  float* scratch_all = reinterpret_cast<float*>(pieces + 2 * kWarps);
+  // the swizzle's exclusive-or works on addresses whose rows begin on 128 bytes
+  unsigned char* smem = smem_any + (-smem_u32(smem_any) & 127u);
+  // rings, then a piece of each warp, then its scratch.  A warp's second piece takes its ring, which is empty by then.
+  Part* first_pieces = reinterpret_cast<Part*>(smem + kWarps * kSlots * kSlotBytes);
+  const auto piece_at = [&](int i) {
+    return i & 1 ? reinterpret_cast<Part*>(smem + (i >> 1) * (kSlots * kSlotBytes)) : first_pieces + (i >> 1);
+  };
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  unsigned char* ring = smem + warp * (kStages * kStageBytes);
-  float* scratch = scratch_all + warp * kScratch;
+  unsigned char* ring = smem + warp * (kSlots * kSlotBytes);
+  float* scratch = reinterpret_cast<float*>(first_pieces + kWarps) + warp * Math::kScratch;
   const int dim = cache.head_dim, items = cache.kv_heads * a.chunks;
   const int live_chunks = dim * static_cast<int>(sizeof(T)) / 16;
   if (live_chunks < kChunks) {  // the columns that no token fills
-    for (int i = lane; i < kStages * kStageBytes / 16; i += 32)
+    for (int i = lane; i < kSlots * kSlotBytes / 16; i += 32)
       reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   if (lane == 0) {
@@ -592,145 +614,179 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args
   __syncthreads();
   long long before = sum - mine, all = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_scan[w];
     all += s_scan[w];
   }
-  const long long total = all * items, workers = static_cast<long long>(gridDim.x) * kWarps;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const long long from = total * (static_cast<long long>(blockIdx.x) * kWarps + w) / workers;
-    if (mine > 0 && from >= before * items && from < (before + mine) * items) {
-      long long at = before;
-      for (int r = r0; r < r1; ++r) {
-        bool b;
-        const int tokens = row_tokens(a, r, &b), tiles = (tokens + kTok - 1) / kTok;
-        if (from < (at + tiles) * items) {
-          const int item = static_cast<int>((from - at * items) / tiles);
-          s_first[w] = Segment{r, item, at * items + static_cast<long long>(item) * tiles, tiles, tokens};
-          break;
+  const long long total = all * items;
+  // CTAs in use: no more than give each of their warps a tile, so that short rows are joined within a CTA
+  const long long wanted = (total + kWarps - 1) / kWarps;
+  const int ctas = wanted < gridDim.x ? static_cast<int>(wanted) : gridDim.x;
+  const int cta = blockIdx.x;
+  const long long workers = static_cast<long long>(ctas) * kWarps;
+  if (cta < ctas) {
+    for (int w = 0; w < kWarps; ++w) {
+      const long long from = total * (static_cast<long long>(cta) * kWarps + w) / workers;
+      if (mine > 0 && from >= before * items && from < (before + mine) * items) {
+        long long at = before;
+        for (int r = r0; r < r1; ++r) {
+          bool b;
+          const int tokens = row_tokens(a, r, &b), tiles = (tokens + kTok - 1) / kTok;
+          if (from < (at + tiles) * items) {
+            const int item = static_cast<int>((from - at * items) / tiles);
+            s_first[w] = Segment{r, item, at * items + static_cast<long long>(item) * tiles, tiles, tokens};
+            break;
+          }
+          at += tiles;
         }
-        at += tiles;
       }
     }
   }
   // rows without tokens
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  for (int r = cta; r < a.rows; r += gridDim.x) {
     bool b;
     if (row_tokens(a, r, &b) == 0)
       for (int i = tid; i < a.heads * dim / 4; i += kThreads)
         reinterpret_cast<float4*>(a.out + r * a.out_stride)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  if (cta >= ctas) return;
   __syncthreads();
 
-  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const long long worker = static_cast<long long>(cta) * kWarps + warp;
   const long long begin = total * worker / workers, end = total * (worker + 1) / workers;
   const auto heads_of = [&](int item) { return min(kGroup, a.group - item % a.chunks * kGroup); };
   const auto head_of = [&](int item) { return item / a.chunks * a.group + item % a.chunks * kGroup; };
 
   if (begin < end) {
-    Walk<kTok> load;
-    load.s = s_first[warp];
-    load.at = begin;
-    load.end = end;
-    // places of the next tile's tokens: 16-byte units from the layer's first element, -1: none
-    long long place[kPer];
+    Segment load = s_first[warp];  // of the tile to be loaded next
+    long long load_at = begin;
+    long long place[kPer];  // bytes from the layer's first element to the lane's tokens of that tile; -1: none
+    unsigned long long live = 0;
     const auto look_up = [&]() {
-      const Segment& s = load.s;
-      const int t0 = static_cast<int>(load.at - s.start) * kTok;
-      const int seq = a.seq ? a.seq[s.row] : s.row;
+      const int t0 = static_cast<int>(load_at - load.start) * kTok;
+      const int seq = a.seq ? a.seq[load.row] : load.row;
       const int* table = a.page_table + seq * a.table_stride;
+      const long long head = load.item / a.chunks * cache.head_stride;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int t = t0 + lane + 32 * i;
         place[i] = -1;
-        if (lane + 32 * i < kTok && t < s.tokens) {
+        if (lane + 32 * i < kTok && t < load.tokens) {
           const unsigned col = divide(t, a.page_div);
           const int page = table[col];
           if (page >= 0 && page < cache.pages)
-            place[i] = page * cache.page_stride + (t - col * a.page_div.by) * cache.slot_stride;
+            place[i] = (page * cache.page_stride + (t - col * a.page_div.by) * cache.slot_stride + head) *
+                       static_cast<long long>(sizeof(T));
           else
             record_device_error(kDevPageRange);
         }
       }
     };
-    const auto issue = [&](int slot) {
-      const Segment& s = load.s;
-      unsigned long long live = 0;
+    const auto advance = [&]() {
+      if (++load_at < load.start + load.tiles || load_at >= end) return;
+      load.start += load.tiles;
+      if (++load.item < items) return;
+      load.item = 0;
+      bool b;
+      do {
+        load.tokens = row_tokens(a, ++load.row, &b);
+      } while (load.tokens == 0 && load.row + 1 < a.rows);
+      load.tiles = (load.tokens + kTok - 1) / kTok;
+    };
+    // One tile's keys or values into a slot: each lane a 16-byte chunk of one row in kAtOnce.
+    constexpr int kAtOnce = kChunks < 32 ? 32 / kChunks : 1, kWide = kChunks > 32 ? kChunks / 32 : 1;
+    const int sub = kChunks < 32 ? lane / kChunks : 0, chunk = lane % kChunks;
+    const unsigned lane_to = sub * kRowBytes + (((chunk & 7) ^ sub) << 4) + ((chunk >> 3) << 7);
+    const auto fill = [&](int slot, const T* from) {
+      const unsigned to = smem_u32(ring) + slot * kSlotBytes + lane_to;
+      const char* src = reinterpret_cast<const char*>(from) + chunk * 16;
+      const auto copy = [&](auto whole) {
+#pragma unroll
+        for (int i = 0; i < kTok / kAtOnce; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, place[i * kAtOnce / 32], (i * kAtOnce + sub) & 31);
+          const unsigned p = swizzled(to, i * kAtOnce & 7) + i * kAtOnce * kRowBytes;
+#pragma unroll
+          for (int j = 0; j < kWide; ++j) {
+            if (chunk + 32 * j >= live_chunks) continue;
+            if constexpr (decltype(whole)::value)
+              cp_async16(p + 512 * j, src + at + 512 * j);
+            else
+              cp_async16(p + 512 * j, src + (at >= 0 ? at : 0) + 512 * j, at >= 0);
+          }
+        }
+      };
+      if (live == kAll)
+        copy(std::true_type());
+      else
+        copy(std::false_type());
+    };
+    const auto find_live = [&]() {
+      live = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         live |= static_cast<unsigned long long>(__ballot_sync(0xffffffffu, place[i] >= 0)) << (32 * i);
-      if (lane == 0) {
-        int flags = 0;
-        if (load.at == s.start || load.at == begin) flags |= kFirst;
-        if (load.at + 1 == s.start + s.tiles || load.at + 1 == end) flags |= kLast;
-        if (s.start >= begin && s.start + s.tiles <= end) flags |= kWhole;
-        s_info[warp][slot] = TileInfo{live, s.start, s.row, s.item, s.tiles, flags};
-      }
-      const long long head = s.item / a.chunks * cache.head_stride;
-      unsigned char* to = ring + slot * kStageBytes;
-      constexpr int kRowsAtOnce = 32 / kChunks > 0 ? 32 / kChunks : 1;
-      constexpr int kWide = kChunks > 32 ? kChunks / 32 : 1;
-      const int chunk = lane % kChunks;
-      constexpr int kVec = 16 / sizeof(T);
-#pragma unroll
-      for (int i = 0; i < kTok / kRowsAtOnce; ++i) {
-        const int t = i * kRowsAtOnce + (kChunks < 32 ? lane / kChunks : 0);
-        const long long at = __shfl_sync(0xffffffffu, place[i * kRowsAtOnce / 32], t & 31);
-        const bool on = at >= 0;
-        const long long off = on ? at + head : 0;
-#pragma unroll
-        for (int j = 0; j < kWide; ++j) {
-          const int k = chunk + 32 * j;
-          if (k < live_chunks) {
-            unsigned char* p = to + (t * kChunks + (k ^ (t & 7))) * 16;
-            cp_async16(p, cache.k + off + k * kVec, on);
-            cp_async16(p + kTok * kChunks * 16, cache.v + off + k * kVec, on);
-          }
-        }
-      }
     };
-    const auto next = [&](int slot) {
-      if (load.at < end) {
-        issue(slot);
-        load.advance(a, items);
-        if (load.at < end) look_up();
+    const auto next_slot = [](int s) { return s + 1 == kSlots ? 0 : s + 1; };
+
+    Math math;
+    look_up();
+    find_live();
+    fill(0, cache.k);
+    cp_async_commit();
+    fill(1, cache.v);
+    cp_async_commit();
+    Segment now = load;
+    unsigned long long now_live = live;
+    advance();
+    if (load_at < end) look_up();
+    int slot = 0;
+    for (long long at = begin; at < end; ++at) {
+      // keys of this tile are here, its values and then the next one's keys are under way
+      cp_async_wait<1>();
+      __syncwarp();
+      const int value_slot = next_slot(slot), free_slot = next_slot(value_slot);
+      const bool more = load_at < end;
+      if (more) {
+        find_live();
+        fill(free_slot, cache.k);
       }
       cp_async_commit();
-    };
-    look_up();
-    for (int i = 0; i < kStages - 1; ++i) next(i);
-    Math math;
-    int slot = 0, ahead = kStages - 1;
-    bool one_held = false;
-    for (long long at = begin; at < end; ++at) {
-      cp_async_wait<kStages - 2>();
+      const int heads = heads_of(now.item);
+      const long long first = static_cast<long long>(head_of(now.item)) * dim;
+      if (at == begin || at == now.start) math.begin(a, a.q + now.row * a.q_stride + first, heads, dim, scratch);
+      math.scores(smem_u32(ring) + slot * kSlotBytes, now_live, scratch);
+      cp_async_wait<1>();
       __syncwarp();
-      const TileInfo info = s_info[warp][slot];
-      next(ahead);
-      const int heads = heads_of(info.item);
-      const long long first = static_cast<long long>(head_of(info.item)) * dim;
-      if (info.flags & kFirst) math.begin(a, a.q + info.row * a.q_stride + first, heads, dim, scratch);
-      math.tile(ring + slot * kStageBytes, info.live, scratch);
-      if (info.flags & kLast) {
-        if (info.flags & kWhole) {
-          math.store(a.out + info.row * a.out_stride + first, heads, dim);
+      const Segment next = load;
+      if (more) fill(slot, cache.v);
+      cp_async_commit();
+      const unsigned long long next_live = live;
+      if (more) {
+        advance();
+        if (load_at < end) look_up();
+      }
+      math.outputs(smem_u32(ring) + value_slot * kSlotBytes, scratch);
+      const long long after = now.start + now.tiles;
+      if (at + 1 == after || at + 1 == end) {
+        if (now.start >= begin && after <= end) {
+          math.store(a.out + now.row * a.out_stride + first, heads, dim);
         } else {
-          const int h = 2 * warp + one_held;
-          one_held = true;
-          math.store(pieces[h]);
-          if (lane == 0) s_held[h] = Held{info.start, info.row, info.item, info.tiles, 1};
+          const int h = 2 * warp + (at + 1 == end);
+          __syncwarp();  // every lane has read its last values
+          math.store(*piece_at(h));
+          if (lane == 0) s_held[h] = Held{now.start, now.row, now.item, now.tiles, 1};
         }
       }
-      slot = slot + 1 == kStages ? 0 : slot + 1;
-      ahead = ahead + 1 == kStages ? 0 : ahead + 1;
+      now = next;
+      now_live = next_live;
+      slot = free_slot;
     }
     cp_async_wait<0>();
   }
   __syncthreads();
 
   // ---- the join -------------------------------------------------------------------
-  const long long cta_begin = total * blockIdx.x / gridDim.x, cta_end = total * (blockIdx.x + 1) / gridDim.x;
+  const long long cta_begin = total * cta / ctas, cta_end = total * (cta + 1) / ctas;
   int p = 0;
   while (p < 2 * kWarps) {
     if (!s_held[p].used) {
@@ -744,15 +800,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args
     const int heads = heads_of(held.item);
     float* out = a.out + held.row * a.out_stride + static_cast<long long>(head_of(held.item)) * dim;
     const bool whole = held.start >= cta_begin && held.start + held.tiles <= cta_end;
-    Piece<kDim>* mine_out =
-        reinterpret_cast<Piece<kDim>*>(a.partials) + 2 * blockIdx.x + (held.start >= cta_begin && held.start != cta_begin ? 1 : 0);
+    Part* parts_of = static_cast<Part*>(a.partials);
+    // a CTA's first segment may have begun before it (slot 0), its last may go on behind it (slot 1)
+    Part* to = parts_of + 2 * cta + (held.start > cta_begin ? 1 : 0);
     for (int i = tid; i < heads * (kDim / 4); i += kThreads) {
       const int h = i / (kDim / 4), e = 4 * (i % (kDim / 4));
       float top = -INFINITY, sum_l = 0.f;
-      for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, pieces[__ffs(b) - 1].m[h]);
+      for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
       for (unsigned b = members; b; b &= b - 1) {
-        const Piece<kDim>& x = pieces[__ffs(b) - 1];
+        const Part& x = *piece_at(__ffs(b) - 1);
         const float w = piece_weight(x.m[h], top, x.c[h]);
         const float4 v = *reinterpret_cast<const float4*>(&x.o[h][e]);
         sum_l = fmaf(w, x.l[h], sum_l);
@@ -763,21 +820,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args
         if (e < dim)
           *reinterpret_cast<float4*>(out + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
       } else {
-        *reinterpret_cast<float4*>(&mine_out->o[h][e]) = y;
+        *reinterpret_cast<float4*>(&to->o[h][e]) = y;
         if (e == 0) {
-          mine_out->m[h] = top;
-          mine_out->l[h] = sum_l;
-          mine_out->c[h] = pieces[__ffs(members) - 1].c[h];
+          to->m[h] = top;
+          to->l[h] = sum_l;
+          to->c[h] = piece_at(__ffs(members) - 1)->c[h];
         }
       }
     }
     if (whole) continue;
-    // the CTAs that hold tiles of the segment: all from the first to the last, or one a tile when there are
-    // more CTAs than tiles
-    const auto cta_of = [&](long long tile) { return ((tile + 1) * gridDim.x - 1) / total; };
-    const long long first_cta = cta_of(held.start);
-    const bool sparse = total < gridDim.x;
-    const int parts = sparse ? held.tiles : static_cast<int>(cta_of(held.start + held.tiles - 1) - first_cta) + 1;
+    // every CTA from that of the segment's first tile to that of its last holds a part
+    const auto cta_of = [&](long long tile) { return static_cast<int>(((tile + 1) * ctas - 1) / total); };
+    const int first_cta = cta_of(held.start);
+    const int parts = cta_of(held.start + held.tiles - 1) - first_cta + 1;
     __syncthreads();
     if (tid == 0) {
       __threadfence();
@@ -788,22 +843,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args
     }
     __syncthreads();
     if (s_last) {
-      const Piece<kDim>* from = reinterpret_cast<const Piece<kDim>*>(a.partials);
-      const auto part = [&](int i) {
-        const long long cta = sparse ? cta_of(held.start + i) : first_cta + i;
-        const long long b = total * cta / gridDim.x;
-        return from + 2 * cta + (held.start > b ? 1 : 0);
-      };
+      // slot 0 of all CTAs but the first, in which the segment may be the last one
+      const Part* first_part =
+          parts_of + 2 * first_cta + (held.start > total * first_cta / ctas ? 1 : 0);
+      const Part* other = parts_of + 2 * first_cta;
       for (int i = tid; i < heads * (kDim / 4); i += kThreads) {
         const int h = i / (kDim / 4), e = 4 * (i % (kDim / 4));
         if (e >= dim) continue;
-        float top = -INFINITY, sum_l = 0.f;
-        for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&part(k)->m[h]));
+        float top = __ldcg(&first_part->m[h]), sum_l = 0.f;
+        const float c = __ldcg(&first_part->c[h]);
+#pragma unroll 8
+        for (int k = 1; k < parts; ++k) top = fmaxf(top, __ldcg(&other[2 * k].m[h]));
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < parts; ++k) {
-          const Piece<kDim>* x = part(k);
-          const float w = piece_weight(__ldcg(&x->m[h]), top, __ldcg(&x->c[h]));
+          const Part* x = k == 0 ? first_part : other + 2 * k;
+          const float w = piece_weight(__ldcg(&x->m[h]), top, c);
           const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
           sum_l = fmaf(w, __ldcg(&x->l[h]), sum_l);
           y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
@@ -816,39 +871,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Args
   }
 }
 
-template <typename Math, typename T, int kDim, int kStages>
-int launch_math(Args a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t stream) {
+template <typename Math, typename T, int kDim>
+int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   const DeviceInfo& dev = current_device(&e);
   if (e != cudaSuccess) return check_cuda(e);
-  const size_t smem = static_cast<size_t>(kWarps) * kStages * kStageBytes + 2 * kWarps * sizeof(Piece<kDim>) +
-                      (sizeof(T) == 4 ? kWarps * (kGroup * kDim + Math::kTok * kGroup) * sizeof(float) : 0);
-  auto kernel = paged_attention_kernel<Math, T, kDim, kStages>;
-  e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  constexpr int kWarps = kWarpsOf<Math>;
+  constexpr size_t kSmem = static_cast<size_t>(kWarps) * kWarpBytes<Math> + 128;
+  auto kernel = paged_attention_kernel<Math, T, kDim>;
+  e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (e != cudaSuccess) return check_cuda(e);
   // no more CTAs than tiles can be
   const long long most = static_cast<long long>(op.rows) * cache.kv_heads * a.chunks;
   const long long tiles = (a.room + Math::kTok - 1) / Math::kTok;
   int grid = dev.sm_count < kMaxCtas ? dev.sm_count : kMaxCtas;
   if (most < grid && most * tiles < grid) grid = static_cast<int>(most * tiles);
-  return check_cuda(launch(kernel, dim3(grid), dim3(kThreads), smem, stream, true, a, cache_layer<T>(cache, layer)));
+  return check_cuda(
+      launch(kernel, dim3(grid), dim3(kWarps * 32), kSmem, stream, true, a, cache_layer<T>(cache, layer)));
 }
 
 template <typename T, int kDim>
 int launch_dim(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
-  // stages: what is left of 227 KB beside the pieces, at most 3
-  constexpr int kStages = kDim == 256 ? 2 : 3;
+  // half of the products where all heads of a pass fit beside their parts
   const bool few = a.group <= 4;
-  if constexpr (sizeof(T) == 4) {
-    constexpr int kFloatStages = 2;
-    return few ? launch_math<FloatMath<kDim, true>, T, kDim, kFloatStages>(a, op, cache, layer, s)
-               : launch_math<FloatMath<kDim, false>, T, kDim, kFloatStages>(a, op, cache, layer, s);
-  } else {
-    return few ? launch_math<TensorMath<T, kDim, true>, T, kDim, kStages>(a, op, cache, layer, s)
-               : launch_math<TensorMath<T, kDim, false>, T, kDim, kStages>(a, op, cache, layer, s);
-  }
+  if constexpr (sizeof(T) == 4)
+    return few ? launch_math<FloatMath<kDim, true>, T, kDim>(a, op, cache, layer, s)
+               : launch_math<FloatMath<kDim, false>, T, kDim>(a, op, cache, layer, s);
+  else
+    return few ? launch_math<TensorMath<T, kDim, true>, T, kDim>(a, op, cache, layer, s)
+               : launch_math<TensorMath<T, kDim, false>, T, kDim>(a, op, cache, layer, s);
 }
-
 template <typename T>
 int launch_attention(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
   return cache.head_dim <= 64    ? launch_dim<T, 64>(a, op, cache, layer, s)
@@ -858,7 +910,7 @@ int launch_attention(const Args& a, const mli_attention_op& op, const mli_kv_cac
 
 // The same for every head size, so that the arrivals' place does not depend on it: what one call leaves
 // in the partial results is never another's counter.
-constexpr size_t kPartialBytes = 2 * kMaxCtas * sizeof(Piece<kMaxHeadDim>);
+constexpr size_t kPartialBytes = 2 * kMaxCtas * sizeof(Piece<kMaxHeadDim, kGroup>);
 
 }  // namespace
 }  // namespace mli
@@ -905,7 +957,7 @@ int mli_paged_attention(const mli_attention_op* op, const mli_kv_cache* cache, i
   a.chunks = (a.group + kGroup - 1) / kGroup;
   a.scale = fmaxf(op->scale * 1.4426950408889634f, FLT_MIN);  // log2(e)
   a.page_div = fast_div(cache->page_size);
-  a.partials = static_cast<float*>(op->workspace);
+  a.partials = op->workspace;
   a.arrivals = reinterpret_cast<unsigned*>(static_cast<char*>(op->workspace) + kPartialBytes);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (cache->dtype) {
