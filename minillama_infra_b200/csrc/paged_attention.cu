@@ -175,42 +175,52 @@ __device__ __forceinline__ unsigned swizzled(unsigned first, int chunk) {
   return (first ^ ((chunk & 7) << 4)) + ((chunk >> 3) << 7);
 }
 
-// kDim: the head dimension's room in shared memory (64, 128 or 256).  kFew: at most 4 heads.
-template <typename T, int kDim, bool kFew>
+// kDim: the head dimension's room in shared memory (64, 128 or 256), the first kUsed of it multiplied.  kFew: at most
+// 4 heads.
+template <typename T, int kDim, int kUsed, bool kFew>
 struct TensorMath {
   static constexpr int kTok = kSlotBytes / (kDim * 2);  // 64, 32 or 16 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kScratch = 0;
-  static constexpr int kSteps = kDim / 16;
+  static constexpr int kSteps = kUsed / 16;
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;
   using Part = Piece<kDim, kHeads>;
 
   unsigned q[kSteps][kFew ? 4 : 6];
   unsigned p[kTok / 8][kFew ? 2 : 3];
-  float2 o[kDim / 8];
+  float2 o[kUsed / 8];
   float m, l, c, keep;
   int head;  // this lane's head within the pass
   bool third;
 
-  __device__ __forceinline__ void begin(const Args& a, const float* qp, int heads, int dim, float*) {
+  // A pass begins: its queries, asked for here and taken apart in begin().
+  struct Queries {
+    float2 x[kSteps][2];
+  };
+  __device__ __forceinline__ void ask(Queries& raw, const float* qp, int heads, int dim) {
     const int lane = threadIdx.x & 31, g = lane >> 2, col = 2 * (lane & 3);
     head = kFew ? g & 3 : g;
     third = kFew && g >= 4;
     const float* row = qp + head * dim;
     const bool live = head < heads;
-    float2 x[kSteps][2];
-    float top = 0.f;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int e = 16 * k + 8 * j + col;
-        x[k][j] = live && e < dim ? *reinterpret_cast<const float2*>(row + e) : make_float2(0.f, 0.f);
-        if (kUp != 1.f) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+        raw.x[k][j] = live && e < dim ? *reinterpret_cast<const float2*>(row + e) : make_float2(0.f, 0.f);
       }
-    c = a.scale;
+  }
+  __device__ __forceinline__ void begin(const Queries& raw, float scale, float*) {
+    c = scale;
     float up = 1.f;
+    const auto& x = raw.x;
     if (kUp != 1.f) {
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int exponent = (__float_as_int(top) >> 23) & 255;
@@ -231,7 +241,7 @@ struct TensorMath {
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i) o[i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < kUsed / 8; ++i) o[i] = make_float2(0.f, 0.f);
   }
 
   // The tile's weights from its keys.  live: bit t for token t.
@@ -299,7 +309,7 @@ struct TensorMath {
     const unsigned row = values + ((mat & 1) * 8 + in) * (kDim * 2) + (((mat >> 1) ^ in) << 4);
     const float2 keep2 = make_float2(keep, keep);
 #pragma unroll
-    for (int d = 0; d < kDim / 16; ++d) {
+    for (int d = 0; d < kSteps; ++d) {
       float acc[2][4];
       const unsigned at = swizzled(row, 2 * d);
 #pragma unroll
@@ -326,7 +336,7 @@ struct TensorMath {
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (kFew) {
 #pragma unroll
-      for (int i = 0; i < kDim / 8; ++i) {
+      for (int i = 0; i < kUsed / 8; ++i) {
         o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, 16);
         o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, 16);
       }
@@ -338,7 +348,7 @@ struct TensorMath {
     const float inv = l == 0.f ? 0.f : 1.f / (l * kUp);
     float* row = out + head * dim + 2 * (threadIdx.x & 3);
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i)
+    for (int i = 0; i < kUsed / 8; ++i)
       if (8 * i < dim) *reinterpret_cast<float2*>(row + 8 * i) = make_float2(o[i].x * inv, o[i].y * inv);
   }
   __device__ __forceinline__ void store(Part& to) {
@@ -346,7 +356,7 @@ struct TensorMath {
     if (third) return;
     const int col = 2 * (threadIdx.x & 3);
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i) *reinterpret_cast<float2*>(&to.o[head][8 * i + col]) = o[i];
+    for (int i = 0; i < kUsed / 8; ++i) *reinterpret_cast<float2*>(&to.o[head][8 * i + col]) = o[i];
     if (col == 0) {
       to.m[head] = m;
       to.l[head] = l * kUp;
@@ -379,17 +389,24 @@ struct FloatMath {
   float2 o[kHeads][kOwn][2];
   float m[kHeads], l[kHeads], keep[kHeads], c;
 
-  __device__ __forceinline__ void begin(const Args& a, const float* qp, int heads, int dim, float* scratch) {
-    const int lane = threadIdx.x & 31;
-    float4* qs = reinterpret_cast<float4*>(scratch);
-    __syncwarp();
-    for (int i = lane; i < kHeads * kChunks; i += 32) {
-      const int h = i / kChunks, e = 4 * (i % kChunks);
-      qs[i] = h < heads && e < dim ? *reinterpret_cast<const float4*>(qp + h * dim + e)
-                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  struct Queries {
+    float4 x[kHeads * kChunks / 32];
+  };
+  __device__ __forceinline__ void ask(Queries& raw, const float* qp, int heads, int dim) {
+#pragma unroll
+    for (int k = 0; k < kHeads * kChunks / 32; ++k) {
+      const int i = (threadIdx.x & 31) + 32 * k, h = i / kChunks, e = 4 * (i % kChunks);
+      raw.x[k] = h < heads && e < dim ? *reinterpret_cast<const float4*>(qp + h * dim + e)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+  }
+  __device__ __forceinline__ void begin(const Queries& raw, float scale, float* scratch) {
     __syncwarp();
-    c = a.scale;
+#pragma unroll
+    for (int k = 0; k < kHeads * kChunks / 32; ++k)
+      reinterpret_cast<float4*>(scratch)[(threadIdx.x & 31) + 32 * k] = raw.x[k];
+    __syncwarp();
+    c = scale;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
       m[h] = -INFINITY;
@@ -522,26 +539,40 @@ struct FloatMath {
 };
 
 // ---- the tiles of a call ---------------------------------------------------------
-// Tokens that row r attends to: its length, cut to the page table; 0 for a row led outside it.
-__device__ __forceinline__ int row_tokens(const Args& a, int r, bool* bad) {
-  const int len = a.lengths[r];
-  if (len <= 0) return 0;
-  if (a.seq != nullptr) {
-    const int s = a.seq[r];
-    if (s < 0 || s >= a.table_rows) {
-      *bad = true;
-      return 0;
-    }
-  }
-  if (len > a.room) *bad = true;
-  return len > a.room ? static_cast<int>(a.room) : len;
+struct Row {
+  int tokens;  // that it attends to: its length, cut to the page table; 0 if its sequence lies outside it
+  int seq;     // its row of the page table
+  bool bad;    // led outside the page table
+};
+__device__ __forceinline__ Row row_of(const Args& a, int r) {
+  const int len = a.lengths[r], seq = a.seq ? a.seq[r] : r;
+  if (len <= 0) return Row{0, 0, false};
+  if (seq < 0 || seq >= a.table_rows) return Row{0, 0, true};
+  return Row{len > a.room ? static_cast<int>(a.room) : len, seq, len > a.room};
+}
+__device__ __forceinline__ long long quotient(long long n, long long by) {  // of numbers >= 0
+  return ((n | by) >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(by) : n / by;
 }
 
 // A segment's place among all tiles.
 struct Segment {
-  int row, item;      // item: key-value head * chunks + chunk
-  long long start;    // first tile
-  int tiles, tokens;
+  long long start;  // first tile
+  int row, item;    // item: key-value head * chunks + chunk
+  int seq, tiles, tokens;
+};
+
+// All tiles in equal shares: the first `more` workers take one more than the others.
+struct Shares {
+  long long each, more;
+  __device__ __forceinline__ Shares(long long total, int workers) {
+    each = quotient(total, workers);
+    more = total - each * workers;
+  }
+  __device__ __forceinline__ long long begin(int worker) const { return worker * each + (worker < more ? worker : more); }
+  __device__ __forceinline__ int worker_of(long long tile) const {
+    const long long longer = more * (each + 1);
+    return static_cast<int>(tile < longer ? quotient(tile, each + 1) : more + quotient(tile - longer, each));
+  }
 };
 
 // A piece that a CTA holds in shared memory.
@@ -551,7 +582,7 @@ struct Held {
 };
 
 // Bytes of a warp, and how many of them an SM's 227 KB hold beside the static arrays and 128 bytes for alignment.
-constexpr int kSmemRoom = 232448 - 1024 - 128;
+constexpr int kSmemRoom = 232448 - 1792 - 128;
 template <typename Math>
 constexpr int kWarpBytes = kSlots * kSlotBytes + sizeof(typename Math::Part) + Math::kScratch * 4;
 template <typename Math>
@@ -569,10 +600,9 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   constexpr unsigned long long kAll = ~0ull >> (64 - kTok);
 
   extern __shared__ unsigned char smem_any[];
-  __shared__ long long s_scan[kWarps];
-  __shared__ Segment s_first[kWarps];
+  __shared__ unsigned s_scan[kWarps], s_before[kThreads];
   __shared__ Held s_held[2 * kWarps];
-  __shared__ int s_last;
+  __shared__ int s_last[2];
   // the swizzle's exclusive-or works on addresses whose rows begin on 128 bytes
   unsigned char* smem = smem_any + (-smem_u32(smem_any) & 127u);
   // rings, then a piece of each warp, then its scratch.  A warp's second piece takes its ring, which is empty by then.
@@ -590,82 +620,84 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     for (int i = lane; i < kSlots * kSlotBytes / 16; i += 32)
       reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  if (lane == 0) {
-    s_held[2 * warp].used = s_held[2 * warp + 1].used = 0;
-    s_first[warp] = Segment{0, 0, 0, 0, 0};
-  }
+  if (lane == 0) s_held[2 * warp].used = s_held[2 * warp + 1].used = 0;
   griddep_wait();
   griddep_launch_dependents();
 
   // Where each warp starts: thread i sums the tiles of rows [i n, (i + 1) n).
   const int n = (a.rows + kThreads - 1) / kThreads;
-  const int r0 = min(a.rows, tid * n), r1 = min(a.rows, r0 + n);
-  long long mine = 0;
-  bool bad = false;
-  for (int r = r0; r < r1; ++r) mine += (row_tokens(a, r, &bad) + kTok - 1) / kTok;
-  if (bad && blockIdx.x == 0) record_device_error(kDevPageRange);
-  long long sum = mine;
+  unsigned mine = 0;
+  {
+    bool bad = false;
+    for (int r = tid * n; r < min(a.rows, (tid + 1) * n); ++r) {
+      const Row row = row_of(a, r);
+      mine += (row.tokens + kTok - 1) / kTok;
+      bad |= row.bad;
+    }
+    if (bad && blockIdx.x == 0) record_device_error(kDevPageRange);
+  }
+  unsigned sum = mine;
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
-    const long long x = __shfl_up_sync(0xffffffffu, sum, off);
+    const unsigned x = __shfl_up_sync(0xffffffffu, sum, off);
     if (lane >= off) sum += x;
   }
   if (lane == 31) s_scan[warp] = sum;
   __syncthreads();
-  long long before = sum - mine, all = 0;
+  unsigned before = sum - mine, all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_scan[w];
     all += s_scan[w];
   }
-  const long long total = all * items;
+  s_before[tid] = before;
+  const long long total = static_cast<long long>(all) * items;
   // CTAs in use: no more than give each of their warps a tile, so that short rows are joined within a CTA
   const long long wanted = (total + kWarps - 1) / kWarps;
   const int ctas = wanted < gridDim.x ? static_cast<int>(wanted) : gridDim.x;
   const int cta = blockIdx.x;
-  const long long workers = static_cast<long long>(ctas) * kWarps;
-  if (cta < ctas) {
-    for (int w = 0; w < kWarps; ++w) {
-      const long long from = total * (static_cast<long long>(cta) * kWarps + w) / workers;
-      if (mine > 0 && from >= before * items && from < (before + mine) * items) {
-        long long at = before;
-        for (int r = r0; r < r1; ++r) {
-          bool b;
-          const int tokens = row_tokens(a, r, &b), tiles = (tokens + kTok - 1) / kTok;
-          if (from < (at + tiles) * items) {
-            const int item = static_cast<int>((from - at * items) / tiles);
-            s_first[w] = Segment{r, item, at * items + static_cast<long long>(item) * tiles, tiles, tokens};
-            break;
-          }
-          at += tiles;
-        }
-      }
-    }
+  const auto clear_empty_rows = [&]() {
+    for (int r = cta; r < a.rows; r += gridDim.x)
+      if (row_of(a, r).tokens == 0)
+        for (int i = tid; i < a.heads * dim / 4; i += kThreads)
+          reinterpret_cast<float4*>(a.out + r * a.out_stride)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  if (cta >= ctas) {
+    clear_empty_rows();
+    return;
   }
-  // rows without tokens
-  for (int r = cta; r < a.rows; r += gridDim.x) {
-    bool b;
-    if (row_tokens(a, r, &b) == 0)
-      for (int i = tid; i < a.heads * dim / 4; i += kThreads)
-        reinterpret_cast<float4*>(a.out + r * a.out_stride)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  if (cta >= ctas) return;
-  __syncthreads();
-
-  const long long worker = static_cast<long long>(cta) * kWarps + warp;
-  const long long begin = total * worker / workers, end = total * (worker + 1) / workers;
+  const Shares shares(total, ctas * kWarps);
+  const long long begin = shares.begin(cta * kWarps + warp), end = shares.begin(cta * kWarps + warp + 1);
   const auto heads_of = [&](int item) { return min(kGroup, a.group - item % a.chunks * kGroup); };
   const auto head_of = [&](int item) { return item / a.chunks * a.group + item % a.chunks * kGroup; };
+  __syncthreads();
 
   if (begin < end) {
-    Segment load = s_first[warp];  // of the tile to be loaded next
+    // the segment of the warp's first tile: in the rows of the last thread that has no more tiles than that before it
+    Segment load;  // of the tile to be loaded next
+    {
+      unsigned at = static_cast<unsigned>(quotient(begin, items));
+      int owner = -1;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) owner += __popc(__ballot_sync(0xffffffffu, s_before[32 * k + lane] <= at));
+      at -= s_before[owner];
+      int r = owner * n;
+      Row row = row_of(a, r);
+      while (at >= static_cast<unsigned>((row.tokens + kTok - 1) / kTok) && r + 1 < a.rows) {
+        at -= (row.tokens + kTok - 1) / kTok;
+        row = row_of(a, ++r);
+      }
+      const int tiles = max(1, (row.tokens + kTok - 1) / kTok);
+      const long long start = (quotient(begin, items) - at) * items;  // of the row's first item
+      const int item = min(items - 1, static_cast<int>(quotient(begin - start, tiles)));
+      load = Segment{start + static_cast<long long>(item) * tiles, r, item, row.seq, tiles, row.tokens};
+    }
     long long load_at = begin;
     long long place[kPer];  // bytes from the layer's first element to the lane's tokens of that tile; -1: none
     unsigned long long live = 0;
     const auto look_up = [&]() {
       const int t0 = static_cast<int>(load_at - load.start) * kTok;
-      const int seq = a.seq ? a.seq[load.row] : load.row;
-      const int* table = a.page_table + seq * a.table_stride;
+      const int* table = a.page_table + load.seq * a.table_stride;
       const long long head = load.item / a.chunks * cache.head_stride;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -687,10 +719,12 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       load.start += load.tiles;
       if (++load.item < items) return;
       load.item = 0;
-      bool b;
+      Row row;
       do {
-        load.tokens = row_tokens(a, ++load.row, &b);
-      } while (load.tokens == 0 && load.row + 1 < a.rows);
+        row = row_of(a, ++load.row);
+      } while (row.tokens == 0 && load.row + 1 < a.rows);
+      load.tokens = row.tokens;
+      load.seq = row.seq;
       load.tiles = (load.tokens + kTok - 1) / kTok;
     };
     // One tile's keys or values into a slot: each lane a 16-byte chunk of one row in kAtOnce.
@@ -729,7 +763,9 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const auto next_slot = [](int s) { return s + 1 == kSlots ? 0 : s + 1; };
 
     Math math;
+    typename Math::Queries raw;
     look_up();
+    math.ask(raw, a.q + load.row * a.q_stride + static_cast<long long>(head_of(load.item)) * dim, heads_of(load.item), dim);
     find_live();
     fill(0, cache.k);
     cp_async_commit();
@@ -741,8 +777,8 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     if (load_at < end) look_up();
     int slot = 0;
     for (long long at = begin; at < end; ++at) {
-      // keys of this tile are here, its values and then the next one's keys are under way
-      cp_async_wait<1>();
+      // a slot is filled again as soon as all lanes are done with it: two tiles' halves are under way while a third
+      // is worked on
       __syncwarp();
       const int value_slot = next_slot(slot), free_slot = next_slot(value_slot);
       const bool more = load_at < end;
@@ -753,9 +789,13 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       cp_async_commit();
       const int heads = heads_of(now.item);
       const long long first = static_cast<long long>(head_of(now.item)) * dim;
-      if (at == begin || at == now.start) math.begin(a, a.q + now.row * a.q_stride + first, heads, dim, scratch);
+      if (at == begin || at == now.start) {
+        if (at != begin) math.ask(raw, a.q + now.row * a.q_stride + first, heads, dim);
+        math.begin(raw, a.scale, scratch);
+      }
+      cp_async_wait<2>();
+      __syncwarp();
       math.scores(smem_u32(ring) + slot * kSlotBytes, now_live, scratch);
-      cp_async_wait<1>();
       __syncwarp();
       const Segment next = load;
       if (more) fill(slot, cache.v);
@@ -765,6 +805,8 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
         advance();
         if (load_at < end) look_up();
       }
+      cp_async_wait<2>();
+      __syncwarp();
       math.outputs(smem_u32(ring) + value_slot * kSlotBytes, scratch);
       const long long after = now.start + now.tiles;
       if (at + 1 == after || at + 1 == end) {
@@ -783,91 +825,106 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     }
     cp_async_wait<0>();
   }
+  clear_empty_rows();
   __syncthreads();
 
   // ---- the join -------------------------------------------------------------------
-  const long long cta_begin = total * cta / ctas, cta_end = total * (cta + 1) / ctas;
-  int p = 0;
-  while (p < 2 * kWarps) {
-    if (!s_held[p].used) {
-      ++p;
-      continue;
+  const long long cta_begin = shares.begin(cta * kWarps), cta_end = shares.begin((cta + 1) * kWarps);
+  // Every warp lists the segments that the CTA holds pieces of: lane i looks at piece i, group g begins at the g-th
+  // piece whose segment is not that of the piece before.
+  Held held = Held{0, 0, 0, 0, 0};
+  if (lane < 2 * kWarps) held = s_held[lane];
+  const unsigned used = __ballot_sync(0xffffffffu, held.used != 0);
+  const unsigned below = used & ((1u << lane) - 1);
+  const long long left = __shfl_sync(0xffffffffu, held.start, below ? 31 - __clz(below) : lane);
+  const unsigned firsts = __ballot_sync(0xffffffffu, held.used != 0 && (below == 0 || left != held.start));
+  const int groups = __popc(firsts);
+  const auto group_lane = [&](int g) {
+    unsigned rest = firsts;
+    for (; g > 0; --g) rest &= rest - 1;
+    return __ffs(rest) - 1;
+  };
+  const auto group_held = [&](int from) {
+    return Held{__shfl_sync(0xffffffffu, held.start, from), __shfl_sync(0xffffffffu, held.row, from),
+                __shfl_sync(0xffffffffu, held.item, from), __shfl_sync(0xffffffffu, held.tiles, from), 1};
+  };
+  const auto out_of = [&](const Held& g) {
+    return a.out + g.row * a.out_stride + static_cast<long long>(head_of(g.item)) * dim;
+  };
+  Part* parts = static_cast<Part*>(a.partials);
+  constexpr int kQuads = kDim / 4, kItems = Math::kHeads * kQuads;  // a group's float4, a multiple of 32
+  for (int i = tid; i < groups * kItems; i += kThreads) {
+    const int from = group_lane(i / kItems);
+    const Held g = group_held(from);
+    const unsigned later = firsts & ~((2u << from) - 1);
+    const unsigned members = used & ~((1u << from) - 1) & (later ? (later & -later) - 1 : ~0u);
+    const int h = i % kItems / kQuads, e = 4 * (i % kQuads);
+    if (h >= heads_of(g.item)) continue;
+    float top = -INFINITY, sum_l = 0.f;
+    for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
+    const float c = piece_at(from)->c[h];
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (unsigned b = members; b; b &= b - 1) {
+      const Part& x = *piece_at(__ffs(b) - 1);
+      const float w = piece_weight(x.m[h], top, c);
+      const float4 v = *reinterpret_cast<const float4*>(&x.o[h][e]);
+      sum_l = fmaf(w, x.l[h], sum_l);
+      y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
     }
-    const Held held = s_held[p];
-    unsigned members = 0;  // this CTA's pieces of the segment
-    for (; p < 2 * kWarps && (!s_held[p].used || s_held[p].start == held.start); ++p)
-      if (s_held[p].used) members |= 1u << p;
-    const int heads = heads_of(held.item);
-    float* out = a.out + held.row * a.out_stride + static_cast<long long>(head_of(held.item)) * dim;
-    const bool whole = held.start >= cta_begin && held.start + held.tiles <= cta_end;
-    Part* parts_of = static_cast<Part*>(a.partials);
-    // a CTA's first segment may have begun before it (slot 0), its last may go on behind it (slot 1)
-    Part* to = parts_of + 2 * cta + (held.start > cta_begin ? 1 : 0);
-    for (int i = tid; i < heads * (kDim / 4); i += kThreads) {
-      const int h = i / (kDim / 4), e = 4 * (i % (kDim / 4));
-      float top = -INFINITY, sum_l = 0.f;
-      for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (unsigned b = members; b; b &= b - 1) {
-        const Part& x = *piece_at(__ffs(b) - 1);
-        const float w = piece_weight(x.m[h], top, x.c[h]);
-        const float4 v = *reinterpret_cast<const float4*>(&x.o[h][e]);
-        sum_l = fmaf(w, x.l[h], sum_l);
-        y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
-      }
-      if (whole) {
-        const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
-        if (e < dim)
-          *reinterpret_cast<float4*>(out + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-      } else {
-        *reinterpret_cast<float4*>(&to->o[h][e]) = y;
-        if (e == 0) {
-          to->m[h] = top;
-          to->l[h] = sum_l;
-          to->c[h] = piece_at(__ffs(members) - 1)->c[h];
-        }
+    if (g.start >= cta_begin && g.start + g.tiles <= cta_end) {
+      const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+      if (e < dim)
+        *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    } else {
+      // a CTA's first segment may have begun before it (slot 0), its last may go on behind it (slot 1)
+      Part* to = parts + 2 * cta + (g.start > cta_begin ? 1 : 0);
+      *reinterpret_cast<float4*>(&to->o[h][e]) = y;
+      if (e == 0) {
+        to->m[h] = top;
+        to->l[h] = sum_l;
+        to->c[h] = c;
       }
     }
-    if (whole) continue;
-    // every CTA from that of the segment's first tile to that of its last holds a part
-    const auto cta_of = [&](long long tile) { return static_cast<int>(((tile + 1) * ctas - 1) / total); };
-    const int first_cta = cta_of(held.start);
-    const int parts = cta_of(held.start + held.tiles - 1) - first_cta + 1;
+  }
+  // Only the first and the last segment can go beyond the CTA; of each, every CTA from that of its first tile to that
+  // of its last holds a part.
+  for (int k = 0; k < min(groups, 2); ++k) {
+    const Held g = group_held(group_lane(k == 0 ? 0 : groups - 1));
+    if (g.start >= cta_begin && g.start + g.tiles <= cta_end) continue;
+    const int first_cta = shares.worker_of(g.start) / kWarps;
+    const int count = shares.worker_of(g.start + g.tiles - 1) / kWarps - first_cta + 1;
     __syncthreads();
     if (tid == 0) {
       __threadfence();
       // wraps to zero at the last arrival: ready for the next call
-      s_last = atomicInc(a.arrivals + static_cast<long long>(held.row) * items + held.item, parts - 1) ==
-               static_cast<unsigned>(parts - 1);
+      s_last[k] = atomicInc(a.arrivals + static_cast<long long>(g.row) * items + g.item, count - 1) ==
+                  static_cast<unsigned>(count - 1);
       __threadfence();
     }
     __syncthreads();
-    if (s_last) {
-      // slot 0 of all CTAs but the first, in which the segment may be the last one
-      const Part* first_part =
-          parts_of + 2 * first_cta + (held.start > total * first_cta / ctas ? 1 : 0);
-      const Part* other = parts_of + 2 * first_cta;
-      for (int i = tid; i < heads * (kDim / 4); i += kThreads) {
-        const int h = i / (kDim / 4), e = 4 * (i % (kDim / 4));
-        if (e >= dim) continue;
-        float top = __ldcg(&first_part->m[h]), sum_l = 0.f;
-        const float c = __ldcg(&first_part->c[h]);
+    if (!s_last[k]) continue;
+    // slot 0 of all CTAs but the first, in which the segment may be the last one
+    const Part* first_part = parts + 2 * first_cta + (g.start > shares.begin(first_cta * kWarps) ? 1 : 0);
+    const Part* other = parts + 2 * first_cta;
+    for (int i = tid; i < heads_of(g.item) * kQuads; i += kThreads) {
+      const int h = i / kQuads, e = 4 * (i % kQuads);
+      if (e >= dim) continue;
+      float top = __ldcg(&first_part->m[h]), sum_l = 0.f;
+      const float c = __ldcg(&first_part->c[h]);
 #pragma unroll 8
-        for (int k = 1; k < parts; ++k) top = fmaxf(top, __ldcg(&other[2 * k].m[h]));
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 1; j < count; ++j) top = fmaxf(top, __ldcg(&other[2 * j].m[h]));
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int k = 0; k < parts; ++k) {
-          const Part* x = k == 0 ? first_part : other + 2 * k;
-          const float w = piece_weight(__ldcg(&x->m[h]), top, c);
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
-          sum_l = fmaf(w, __ldcg(&x->l[h]), sum_l);
-          y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
-        }
-        const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
-        *reinterpret_cast<float4*>(out + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+      for (int j = 0; j < count; ++j) {
+        const Part* x = j == 0 ? first_part : other + 2 * j;
+        const float w = piece_weight(__ldcg(&x->m[h]), top, c);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
+        sum_l = fmaf(w, __ldcg(&x->l[h]), sum_l);
+        y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
       }
+      const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+      *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
     }
-    __syncthreads();
   }
 }
 
@@ -881,16 +938,17 @@ int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& c
   auto kernel = paged_attention_kernel<Math, T, kDim>;
   e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (e != cudaSuccess) return check_cuda(e);
-  // no more CTAs than tiles can be
   const long long most = static_cast<long long>(op.rows) * cache.kv_heads * a.chunks;
   const long long tiles = (a.room + Math::kTok - 1) / Math::kTok;
+  if (op.rows * tiles >> 32) return set_status(MLI_ERR_UNSUPPORTED);  // tiles are counted in 32 bits
+  // no more CTAs than tiles can be
   int grid = dev.sm_count < kMaxCtas ? dev.sm_count : kMaxCtas;
   if (most < grid && most * tiles < grid) grid = static_cast<int>(most * tiles);
   return check_cuda(
       launch(kernel, dim3(grid), dim3(kWarps * 32), kSmem, stream, true, a, cache_layer<T>(cache, layer)));
 }
 
-template <typename T, int kDim>
+template <typename T, int kDim, int kUsed>
 int launch_dim(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
   // half of the products where all heads of a pass fit beside their parts
   const bool few = a.group <= 4;
@@ -898,14 +956,21 @@ int launch_dim(const Args& a, const mli_attention_op& op, const mli_kv_cache& ca
     return few ? launch_math<FloatMath<kDim, true>, T, kDim>(a, op, cache, layer, s)
                : launch_math<FloatMath<kDim, false>, T, kDim>(a, op, cache, layer, s);
   else
-    return few ? launch_math<TensorMath<T, kDim, true>, T, kDim>(a, op, cache, layer, s)
-               : launch_math<TensorMath<T, kDim, false>, T, kDim>(a, op, cache, layer, s);
+    return few ? launch_math<TensorMath<T, kDim, kUsed, true>, T, kDim>(a, op, cache, layer, s)
+               : launch_math<TensorMath<T, kDim, kUsed, false>, T, kDim>(a, op, cache, layer, s);
 }
+
 template <typename T>
 int launch_attention(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
-  return cache.head_dim <= 64    ? launch_dim<T, 64>(a, op, cache, layer, s)
-         : cache.head_dim <= 128 ? launch_dim<T, 128>(a, op, cache, layer, s)
-                                 : launch_dim<T, 256>(a, op, cache, layer, s);
+  const int dim = cache.head_dim;
+  if (dim <= 64) return launch_dim<T, 64, 64>(a, op, cache, layer, s);
+  // the tensor cores' share of a call goes by the dims they multiply: 80 and 96 have kernels of their own
+  if constexpr (sizeof(T) == 2) {
+    if (dim <= 80) return launch_dim<T, 128, 80>(a, op, cache, layer, s);
+    if (dim <= 96) return launch_dim<T, 128, 96>(a, op, cache, layer, s);
+  }
+  if (dim <= 128) return launch_dim<T, 128, 128>(a, op, cache, layer, s);
+  return launch_dim<T, 256, 256>(a, op, cache, layer, s);
 }
 
 // The same for every head size, so that the arrivals' place does not depend on it: what one call leaves
