@@ -561,16 +561,17 @@ struct Segment {
   int seq, tiles, tokens;
 };
 
-// All tiles in equal shares: the first `more` workers take one more than the others.
+// All tiles in equal shares: the first `more` of `among` take one more than the others.
 struct Shares {
-  long long each, more;
-  __device__ __forceinline__ Shares(long long total, int workers) {
-    each = quotient(total, workers);
-    more = total - each * workers;
+  long long first, each, more;
+  __device__ __forceinline__ Shares(long long from, long long to, int among) : first(from) {
+    each = quotient(to - from, among);
+    more = to - from - each * among;
   }
-  __device__ __forceinline__ long long begin(int worker) const { return worker * each + (worker < more ? worker : more); }
-  __device__ __forceinline__ int worker_of(long long tile) const {
+  __device__ __forceinline__ long long begin(int i) const { return first + i * each + (i < more ? i : more); }
+  __device__ __forceinline__ int owner(long long tile) const {
     const long long longer = more * (each + 1);
+    tile -= first;
     return static_cast<int>(tile < longer ? quotient(tile, each + 1) : more + quotient(tile - longer, each));
   }
 };
@@ -666,8 +667,10 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     clear_empty_rows();
     return;
   }
-  const Shares shares(total, ctas * kWarps);
-  const long long begin = shares.begin(cta * kWarps + warp), end = shares.begin(cta * kWarps + warp + 1);
+  const Shares shares(0, total, ctas);
+  const long long cta_begin = shares.begin(cta), cta_end = shares.begin(cta + 1);
+  const Shares warp_shares(cta_begin, cta_end, kWarps);
+  const long long begin = warp_shares.begin(warp), end = warp_shares.begin(warp + 1);
   const auto heads_of = [&](int item) { return min(kGroup, a.group - item % a.chunks * kGroup); };
   const auto head_of = [&](int item) { return item / a.chunks * a.group + item % a.chunks * kGroup; };
   __syncthreads();
@@ -829,7 +832,6 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   __syncthreads();
 
   // ---- the join -------------------------------------------------------------------
-  const long long cta_begin = shares.begin(cta * kWarps), cta_end = shares.begin((cta + 1) * kWarps);
   // Every warp lists the segments that the CTA holds pieces of: lane i looks at piece i, group g begins at the g-th
   // piece whose segment is not that of the piece before.
   Held held = Held{0, 0, 0, 0, 0};
@@ -887,44 +889,51 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     }
   }
   // Only the first and the last segment can go beyond the CTA; of each, every CTA from that of its first tile to that
-  // of its last holds a part.
-  for (int k = 0; k < min(groups, 2); ++k) {
-    const Held g = group_held(group_lane(k == 0 ? 0 : groups - 1));
-    if (g.start >= cta_begin && g.start + g.tiles <= cta_end) continue;
-    const int first_cta = shares.worker_of(g.start) / kWarps;
-    const int count = shares.worker_of(g.start + g.tiles - 1) / kWarps - first_cta + 1;
-    __syncthreads();
-    if (tid == 0) {
+  // of its last holds a part.  The last of them to get here joins them, in order.
+  const auto end_group = [&](int k) { return group_held(group_lane(k == 0 ? 0 : groups - 1)); };
+  const auto beyond = [&](const Held& g) { return g.start < cta_begin || g.start + g.tiles > cta_end; };
+  const Held ends[2] = {end_group(0), end_group(1)};
+  const bool shared[2] = {groups > 0 && beyond(ends[0]), groups > 1 && beyond(ends[1])};
+  if (!shared[0] && !shared[1]) return;
+  __syncthreads();
+  if (tid < 2) {
+    const Held g = tid == 0 ? ends[0] : ends[1];
+    bool last = false;
+    if (tid == 0 ? shared[0] : shared[1]) {
+      const unsigned most = shares.owner(g.start + g.tiles - 1) - shares.owner(g.start);
       __threadfence();
       // wraps to zero at the last arrival: ready for the next call
-      s_last[k] = atomicInc(a.arrivals + static_cast<long long>(g.row) * items + g.item, count - 1) ==
-                  static_cast<unsigned>(count - 1);
+      last = atomicInc(a.arrivals + static_cast<long long>(g.row) * items + g.item, most) == most;
       __threadfence();
     }
-    __syncthreads();
-    if (!s_last[k]) continue;
+    s_last[tid] = last;
+  }
+  __syncthreads();
+  for (int i = tid; i < 2 * kItems; i += kThreads) {
+    const int k = i / kItems, h = i % kItems / kQuads, e = 4 * (i % kQuads);
+    const Held& g = k == 0 ? ends[0] : ends[1];
+    if (!s_last[k] || h >= heads_of(g.item) || e >= dim) continue;
+    const int first_cta = shares.owner(g.start), count = shares.owner(g.start + g.tiles - 1) - first_cta + 1;
     // slot 0 of all CTAs but the first, in which the segment may be the last one
-    const Part* first_part = parts + 2 * first_cta + (g.start > shares.begin(first_cta * kWarps) ? 1 : 0);
     const Part* other = parts + 2 * first_cta;
-    for (int i = tid; i < heads_of(g.item) * kQuads; i += kThreads) {
-      const int h = i / kQuads, e = 4 * (i % kQuads);
-      if (e >= dim) continue;
-      float top = __ldcg(&first_part->m[h]), sum_l = 0.f;
-      const float c = __ldcg(&first_part->c[h]);
+    const Part* first_part = other + (g.start > shares.begin(first_cta) ? 1 : 0);
+    const float c = __ldcg(&first_part->c[h]);
+    float top = -INFINITY, sum_l = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-      for (int j = 1; j < count; ++j) top = fmaxf(top, __ldcg(&other[2 * j].m[h]));
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int j = 0; j < count; ++j) {
-        const Part* x = j == 0 ? first_part : other + 2 * j;
-        const float w = piece_weight(__ldcg(&x->m[h]), top, c);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
-        sum_l = fmaf(w, __ldcg(&x->l[h]), sum_l);
-        y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
-      }
-      const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
-      *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    for (int j = 0; j < count; ++j) {
+      const Part* x = j == 0 ? first_part : other + 2 * j;
+      const float m = __ldcg(&x->m[h]), l = __ldcg(&x->l[h]);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
+      const float both = fmaxf(top, m);
+      const float keep = piece_weight(top, both, c), w = piece_weight(m, both, c);
+      top = both;
+      sum_l = fmaf(sum_l, keep, w * l);
+      y = make_float4(fmaf(y.x, keep, w * v.x), fmaf(y.y, keep, w * v.y), fmaf(y.z, keep, w * v.z),
+                      fmaf(y.w, keep, w * v.w));
     }
+    const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+    *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
 }
 
