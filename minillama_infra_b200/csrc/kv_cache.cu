@@ -12,19 +12,75 @@
 namespace mli {
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendWarps = 4;
+constexpr int kAppendThreads = kAppendWarps * 32;
+constexpr int kBatch = 4;  // heads whose values a lane holds at once
 
-// One CTA per token: cosine and sine of the token's pairs go to shared memory,
-// then each warp takes heads of q, k and v in turn.
+// Where the other value of a rotated pair comes from.
+enum Partner {
+  kSameQuad,   // interleaved pairs: the same four values
+  kOtherLane,  // halves of whole quads, one quad a lane
+  kOtherQuad,  // halves of 32 quads, two quads a lane
+  kReload,     // any other half: read again
+};
+
+__device__ __forceinline__ void store4(float* p, const float (&y)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+}
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
+__device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
+  __align__(8) T v[4] = {from_float<T>(y[0]), from_float<T>(y[1]), from_float<T>(y[2]), from_float<T>(y[3])};
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+}
+
+// A pass over memory: a token's heads are read once, 16 bytes a lane, and written once.  2^shift lanes hold a head,
+// kQuads times four values each; a warp's heads go in batches whose reads are all under way while the CTA computes
+// its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
+// values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
+template <typename T, int kQuads>
+__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c,
+                                                                     int shift, Partner partner) {
   __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
   griddep_wait();
   griddep_launch_dependents();
   const int t = blockIdx.x;
   const int pos = op.pos[t];
   if (pos < 0) return;  // padding
-  const int half = op.rot_dim / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lanes = 1 << shift, l = lane & (lanes - 1), sub = lane >> shift;
+  const int dim = c.head_dim, half = op.rot_dim / 2, total = op.heads + 2 * c.kv_heads;
+  const int at_once = 32 >> shift, step = gridDim.y * kAppendWarps * at_once;
+
+  const auto source = [&](int h) {
+    return h < op.heads                ? op.q + t * op.q_stride + static_cast<long long>(h) * dim
+           : h < op.heads + c.kv_heads ? op.k + t * op.k_stride + static_cast<long long>(h - op.heads) * dim
+                                       : op.v + t * op.v_stride + static_cast<long long>(h - op.heads - c.kv_heads) * dim;
+  };
+  float4 x[kBatch][kQuads];
+  const auto read = [&](int first) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = first + b * step + sub;
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        const int e = 4 * (l + 32 * i);
+        x[b][i] = h < total && e < dim ? *reinterpret_cast<const float4*>(source(h) + e)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  };
+  int first = (blockIdx.y * kAppendWarps + warp) * at_once;
+  read(first);
+
+  // the token's slot, or -1
+  long long slot = -1;
+  const int seq = op.seq ? op.seq[t] : t;
+  if (seq >= 0 && seq < op.table_rows && pos / c.page_size < op.table_cols) {
+    const int page = op.page_table[seq * op.table_stride + pos / c.page_size];
+    if (page >= 0 && page < c.pages) slot = page * c.page_stride + (pos % c.page_size) * c.slot_stride;
+  }
+  if (slot < 0 && threadIdx.x == 0 && blockIdx.y == 0) record_device_error(kDevPageRange);
+
   for (int i = threadIdx.x; i < half; i += kAppendThreads) {
     // the angle's whole turns are dropped in 64 bits: 2^31 positions leave 22 bits of a turn's fraction
     const double turn = pos * op.turns[i];
@@ -33,84 +89,122 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const mli_r
     s_cos[i] = op.amplitude * co;
     s_sin[i] = op.amplitude * s;
   }
-  // the token's slot, or -1
-  long long slot = -1;
-  const int seq = op.seq ? op.seq[t] : t;
-  if (seq >= 0 && seq < op.table_rows && pos / c.page_size < op.table_cols) {
-    const int page = op.page_table[seq * op.table_stride + pos / c.page_size];
-    if (page >= 0 && page < c.pages) slot = page * c.page_stride + (pos % c.page_size) * c.slot_stride;
-  }
-  if (slot < 0 && threadIdx.x == 0) record_device_error(kDevPageRange);
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const int dim = c.head_dim;
-  for (int h = threadIdx.x >> 5; h < op.heads + 2 * c.kv_heads; h += kAppendThreads / 32) {
-    const bool is_q = h < op.heads;
-    const int hk = is_q ? 0 : (h - op.heads) % c.kv_heads;
-    const bool is_v = h >= op.heads + c.kv_heads;
-    if (!is_q && slot < 0) break;
-    const float* x = is_q ? op.q + t * op.q_stride + static_cast<long long>(h) * dim
-                          : (is_v ? op.v + t * op.v_stride : op.k + t * op.k_stride) + hk * dim;
-    T* to = is_q ? nullptr : (is_v ? c.v : c.k) + slot + hk * c.head_stride;
-    float* qo = op.q_out + t * op.q_out_stride + static_cast<long long>(h) * dim;
-    if (is_v) {
-      for (int e = lane; e < dim; e += 32) to[e] = from_float<T>(x[e]);
-      continue;
-    }
-    const float* w = is_q ? op.q_norm : op.k_norm;
-    float inv = 1.f;
-    if (w) {
-      float ss = 0.f;
-      for (int e = lane; e < dim; e += 32) ss += x[e] * x[e];
-      inv = 1.f / sqrtf(warp_sum(ss) / dim + op.eps);
-    }
-    float y[kMaxHeadDim / 32];
+  // a value y of a pair becomes y cs + (the other) sn; values behind rot_dim: y 1 + 0 0
+  float cs[kQuads][4], sn[kQuads][4];
 #pragma unroll
-    for (int k = 0; k < kMaxHeadDim / 32; ++k) {
-      const int e = lane + 32 * k;
-      if (e >= dim) break;
-      float a = x[e] * inv;
-      if (w) a *= w[e];
-      if (e < op.rot_dim) {
-        const int i = op.interleaved ? e >> 1 : (e < half ? e : e - half);
-        const bool second = op.interleaved ? (e & 1) : e >= half;
-        const int o = op.interleaved ? e ^ 1 : (second ? e - half : e + half);
-        float b = x[o] * inv;
-        if (w) b *= w[o];
-        a = second ? a * s_cos[i] + b * s_sin[i] : a * s_cos[i] - b * s_sin[i];
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = 4 * (l + 32 * i) + j;
+      const bool on = e < op.rot_dim;
+      const bool second = op.interleaved ? (e & 1) : e >= half;
+      const int pair = !on ? 0 : op.interleaved ? e >> 1 : second ? e - half : e;
+      cs[i][j] = on ? s_cos[pair] : 1.f;
+      sn[i][j] = on ? (second ? s_sin[pair] : -s_sin[pair]) : 0.f;
+    }
+
+  while (first < total) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = first + b * step + sub;
+      const bool is_v = h >= op.heads + c.kv_heads;
+      const float* w = h < op.heads ? op.q_norm : is_v ? nullptr : op.k_norm;
+      float inv = 1.f;
+      if (op.q_norm || op.k_norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+          ss += (x[b][i].x * x[b][i].x + x[b][i].y * x[b][i].y) + (x[b][i].z * x[b][i].z + x[b][i].w * x[b][i].w);
+        for (int off = lanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (w) inv = 1.f / sqrtf(ss / dim + op.eps);
       }
-      y[k] = a;
-    }
-    __syncwarp();  // q_out may be q
+      float y[kQuads][4], other[kQuads][4];
 #pragma unroll
-    for (int k = 0; k < kMaxHeadDim / 32; ++k) {
-      const int e = lane + 32 * k;
-      if (e >= dim) break;
-      if (is_q)
-        qo[e] = y[k];
-      else
-        to[e] = from_float<T>(y[k]);
+      for (int i = 0; i < kQuads; ++i) {
+        const int e = 4 * (l + 32 * i);
+        const float4 u = w && e < dim ? *reinterpret_cast<const float4*>(w + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+        y[i][0] = x[b][i].x * inv * u.x;
+        y[i][1] = x[b][i].y * inv * u.y;
+        y[i][2] = x[b][i].z * inv * u.z;
+        y[i][3] = x[b][i].w * inv * u.w;
+      }
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = 4 * (l + 32 * i) + j;
+          if (partner == kSameQuad) {
+            other[i][j] = y[i][j ^ 1];
+          } else if (kQuads == 1 && partner == kOtherLane) {
+            other[i][j] = __shfl_sync(0xffffffffu, y[i][j], l < half / 4 ? l + half / 4 : l - half / 4, lanes);
+          } else if (kQuads == 2 && partner == kOtherQuad) {
+            other[i][j] = y[i ^ 1][j];
+          } else {
+            const int o = e < half ? e + half : e - half;
+            other[i][j] = h < total && !is_v && e < op.rot_dim ? source(h)[o] * inv * (w ? w[o] : 1.f) : 0.f;
+          }
+          if (e >= op.rot_dim) other[i][j] = 0.f;
+        }
+      __syncwarp();  // q_out may be q, whose values a neighbour reads again
+      if (h < total && (h < op.heads || slot >= 0)) {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+          const int e = 4 * (l + 32 * i);
+          if (e >= dim) continue;
+          float z[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[j] = is_v ? y[i][j] : fmaf(y[i][j], cs[i][j], other[i][j] * sn[i][j]);
+          if (h < op.heads)
+            store4(op.q_out + t * op.q_out_stride + static_cast<long long>(h) * dim + e, z);
+          else if (!is_v)
+            store4(c.k + slot + (h - op.heads) * c.head_stride + e, z);
+          else
+            store4(c.v + slot + (h - op.heads - c.kv_heads) * c.head_stride + e, z);
+        }
+      }
     }
+    first += kBatch * step;
+    read(first);
   }
 }
 
 template <typename T>
 int launch_append(const mli_rope_op& op, const mli_kv_cache& cache, int layer, cudaStream_t stream) {
-  return check_cuda(launch(rope_append_kernel<T>, dim3(static_cast<unsigned>(op.m)), dim3(kAppendThreads), 0, stream,
-                           true, op, cache_layer<T>(cache, layer)));
+  cudaError_t e = cudaSuccess;
+  const DeviceInfo& dev = current_device(&e);
+  if (e != cudaSuccess) return check_cuda(e);
+  int shift = 0;
+  while (shift < 5 && (4 << shift) < cache.head_dim) ++shift;
+  const int half = op.rot_dim / 2;
+  const bool wide = cache.head_dim > 128;
+  const Partner partner = op.interleaved || half == 0 ? kSameQuad
+                          : !wide && half % 4 == 0    ? kOtherLane
+                          : wide && half == 128       ? kOtherQuad
+                                                      : kReload;
+  // few tokens: their heads over as many CTAs as give each warp one turn, or as fill the SMs four times
+  const int at_once = kAppendWarps * (32 >> shift), heads = op.heads + 2 * cache.kv_heads;
+  const int most = (heads + at_once - 1) / at_once, fill = 4 * dev.sm_count / op.m;
+  const int share = fill < 1 ? 1 : fill < most ? fill : most;
+  const dim3 grid(static_cast<unsigned>(op.m), static_cast<unsigned>(share));
+  return check_cuda(launch(wide ? rope_append_kernel<T, 2> : rope_append_kernel<T, 1>, grid, dim3(kAppendThreads), 0,
+                           stream, true, op, cache_layer<T>(cache, layer), shift, partner));
 }
 
 constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 8;  // reads of a thread under way at once: 32 KB a CTA
 
+// A page as rows of contiguous 16-byte pieces: row r of `outer` x `inner` begins at (r / inner) * outer_stride +
+// (r % inner) * inner_stride.
 struct CopyArgs {
   uint4* k;
   uint4* v;
-  // in 16-byte units
-  long long layer_stride, page_stride, head_stride, slot_stride;
-  int pages, heads, slots, vecs;  // vecs: 16-byte pieces of one head's slot
+  long long layer_stride, page_stride, outer_stride, inner_stride;  // in 16-byte pieces
+  int pages, inner, row, total;                                     // pieces of a row, of a page
 };
 
-// One CTA per (pair, layer, keys or values).
+// One CTA per (pair, layer, keys or values); bound by HBM, reads and writes alike.
+template <bool kWhole>  // a page is one row
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs a, const int* src, const int* dst) {
   griddep_wait();
   griddep_launch_dependents();
@@ -123,12 +217,23 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs
   uint4* base = (blockIdx.z ? a.v : a.k) + blockIdx.y * a.layer_stride;
   const uint4* p = base + from * a.page_stride;
   uint4* q = base + to * a.page_stride;
-  const int rows = a.slots * a.vecs;
-  for (int h = 0; h < a.heads; ++h)
-    for (int i = threadIdx.x; i < rows; i += kCopyThreads) {
-      const long long off = h * a.head_stride + (i / a.vecs) * a.slot_stride + i % a.vecs;
-      q[off] = p[off];
+  for (int i0 = threadIdx.x; i0 < a.total; i0 += kCopyUnroll * kCopyThreads) {
+    uint4 x[kCopyUnroll];
+    long long off[kCopyUnroll];
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) {
+      const int i = i0 + u * kCopyThreads;
+      if (i >= a.total) break;
+      const int r = kWhole ? 0 : i / a.row;
+      off[u] = kWhole ? i : (r / a.inner) * a.outer_stride + (r % a.inner) * a.inner_stride + i % a.row;
+      x[u] = __ldcs(p + off[u]);
     }
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) {
+      if (i0 + u * kCopyThreads >= a.total) break;
+      __stcs(q + off[u], x[u]);
+    }
+  }
 }
 
 }  // namespace
@@ -198,12 +303,30 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
 int mli_kv_copy_pages(const mli_kv_cache* cache, const int* src, const int* dst, int n, void* stream) {
   const int bad = check_cache(cache);
   if (bad == MLI_ERR_INVALID_ARG || !src || !dst || n <= 0) return set_status(MLI_ERR_INVALID_ARG);
-  if (bad != MLI_OK || cache->layers > 65535) return set_status(MLI_ERR_UNSUPPORTED);
-  const int per = 16 / cache_element_bytes(cache->dtype);
-  const CopyArgs a{static_cast<uint4*>(cache->k), static_cast<uint4*>(cache->v),
-                   cache->layer_stride / per, cache->page_stride / per, cache->head_stride / per,
-                   cache->slot_stride / per, cache->pages, cache->kv_heads, cache->page_size, cache->head_dim / per};
-  return check_cuda(launch(copy_pages_kernel, dim3(static_cast<unsigned>(n), cache->layers, 2), dim3(kCopyThreads), 0,
+  // pieces of a page are counted in 32 bits
+  if (bad != MLI_OK || cache->layers > 65535 ||
+      static_cast<long long>(cache->kv_heads) * cache->page_size > (1 << 24))
+    return set_status(MLI_ERR_UNSUPPORTED);
+  const int per = 16 / cache_element_bytes(cache->dtype), vecs = cache->head_dim / per;
+  const long long head = cache->head_stride / per, slot = cache->slot_stride / per;
+  CopyArgs a{static_cast<uint4*>(cache->k), static_cast<uint4*>(cache->v), cache->layer_stride / per,
+             cache->page_stride / per, head, slot, cache->pages, cache->page_size, vecs,
+             cache->kv_heads * cache->page_size * vecs};
+  // contiguous slots of a head, or heads of a slot, are one row; and all of them together, where they follow one another
+  if (slot == vecs || cache->page_size == 1) {
+    a.row *= cache->page_size;
+    a.inner = 1;
+    a.inner_stride = 0;
+    if (head == a.row || cache->kv_heads == 1) a.row = a.total;
+  } else if (head == vecs || cache->kv_heads == 1) {
+    a.row *= cache->kv_heads;
+    a.inner = 1;
+    a.inner_stride = 0;
+    a.outer_stride = slot;
+    if (slot == a.row) a.row = a.total;
+  }
+  return check_cuda(launch(a.row == a.total ? copy_pages_kernel<true> : copy_pages_kernel<false>,
+                           dim3(static_cast<unsigned>(n), cache->layers, 2), dim3(kCopyThreads), 0,
                            static_cast<cudaStream_t>(stream), true, a, src, dst));
 }
 

@@ -69,6 +69,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// atomicInc that publishes what the CTA wrote before a barrier, and sees what earlier arrivals published.
+__device__ __forceinline__ unsigned arrive(unsigned* p, unsigned most) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(most) : "memory");
+  return old;
+}
+
 struct Args {
   const float* q;
   float* out;
@@ -862,17 +869,22 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const unsigned members = used & ~((1u << from) - 1) & (later ? (later & -later) - 1 : ~0u);
     const int h = i % kItems / kQuads, e = 4 * (i % kQuads);
     if (h >= heads_of(g.item)) continue;
-    float top = -INFINITY, sum_l = 0.f;
-    for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
+    // all pieces' reads at once, those of others left out
+    float m[2 * kWarps], top = -INFINITY, sum_l = 0.f;
     const float c = piece_at(from)->c[h];
+#pragma unroll
+    for (int j = 0; j < 2 * kWarps; ++j) m[j] = (members >> j) & 1 ? piece_at(j)->m[h] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2 * kWarps; ++j) top = fmaxf(top, m[j]);
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (unsigned b = members; b; b &= b - 1) {
-      const Part& x = *piece_at(__ffs(b) - 1);
-      const float w = piece_weight(x.m[h], top, c);
-      const float4 v = *reinterpret_cast<const float4*>(&x.o[h][e]);
-      sum_l = fmaf(w, x.l[h], sum_l);
-      y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
-    }
+#pragma unroll
+    for (int j = 0; j < 2 * kWarps; ++j)
+      if ((members >> j) & 1) {
+        const float w = piece_weight(m[j], top, c);
+        const float4 v = *reinterpret_cast<const float4*>(&piece_at(j)->o[h][e]);
+        sum_l = fmaf(w, piece_at(j)->l[h], sum_l);
+        y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
+      }
     if (g.start >= cta_begin && g.start + g.tiles <= cta_end) {
       const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
       if (e < dim)
@@ -901,10 +913,8 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     bool last = false;
     if (tid == 0 ? shared[0] : shared[1]) {
       const unsigned most = shares.owner(g.start + g.tiles - 1) - shares.owner(g.start);
-      __threadfence();
       // wraps to zero at the last arrival: ready for the next call
-      last = atomicInc(a.arrivals + static_cast<long long>(g.row) * items + g.item, most) == most;
-      __threadfence();
+      last = arrive(a.arrivals + static_cast<long long>(g.row) * items + g.item, most) == most;
     }
     s_last[tid] = last;
   }
@@ -920,17 +930,27 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const float c = __ldcg(&first_part->c[h]);
     float top = -INFINITY, sum_l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int j = 0; j < count; ++j) {
-      const Part* x = j == 0 ? first_part : other + 2 * j;
-      const float m = __ldcg(&x->m[h]), l = __ldcg(&x->l[h]);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
-      const float both = fmaxf(top, m);
-      const float keep = piece_weight(top, both, c), w = piece_weight(m, both, c);
-      top = both;
-      sum_l = fmaf(sum_l, keep, w * l);
-      y = make_float4(fmaf(y.x, keep, w * v.x), fmaf(y.y, keep, w * v.y), fmaf(y.z, keep, w * v.z),
-                      fmaf(y.w, keep, w * v.w));
+    constexpr int kBatch = 4;  // parts read at once
+    for (int j0 = 0; j0 < count; j0 += kBatch) {
+      float m[kBatch], l[kBatch];
+      float4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const Part* x = j0 + j == 0 ? first_part : other + 2 * min(j0 + j, count - 1);
+        m[j] = __ldcg(&x->m[h]);
+        l[j] = __ldcg(&x->l[h]);
+        v[j] = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (j0 + j >= count) break;
+        const float both = fmaxf(top, m[j]);
+        const float keep = piece_weight(top, both, c), w = piece_weight(m[j], both, c);
+        top = both;
+        sum_l = fmaf(sum_l, keep, w * l[j]);
+        y = make_float4(fmaf(y.x, keep, w * v[j].x), fmaf(y.y, keep, w * v[j].y), fmaf(y.z, keep, w * v[j].z),
+                        fmaf(y.w, keep, w * v[j].w));
+      }
     }
     const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
     *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);

@@ -15,6 +15,7 @@ call raises MliError.  torch is used only as a device-memory container.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from ._lib import AttentionOp, GemvOp, KvCacheDesc, RopeOp, check, lib
 
@@ -300,8 +301,27 @@ class GemvChain:
 
 
 # ---- attention over a paged key-value cache ---------------------------------
-_KV_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+# These calls sit on a decode step's host path, many a token: their checks ask each tensor as little as will do.
 _ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
+_ROPE_FIELDS = struct.Struct("@4i2f5P4q5P2iq")
+_ATTENTION_FIELDS = struct.Struct("@2if2P2q3P2iqPN")
+assert _ROPE_FIELDS.size == ctypes.sizeof(RopeOp) and _ATTENTION_FIELDS.size == ctypes.sizeof(AttentionOp)
+
+
+class _Torch:
+    """The parts of torch that every call needs, looked up with the first KvCache."""
+    f32 = f64 = i32 = u8 = device = stream = kv_dtypes = None
+
+    @classmethod
+    def load(cls):
+        import torch
+
+        cls.f32, cls.f64, cls.i32, cls.u8 = torch.float32, torch.float64, torch.int32, torch.uint8
+        cls.kv_dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        # the plain forms of current_device() and current_stream(), which build objects
+        cls.device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        cls.stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                             lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class KvCache:
@@ -315,10 +335,11 @@ class KvCache:
     """
 
     def __init__(self, k, v):
+        _Torch.load()
         if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("expected k and v of one shape [layers, pages, kv_heads, page_size, head_dim], "
                              "one type and one device")
-        if str(k.dtype) not in _KV_DTYPES:
+        if k.dtype not in _Torch.kv_dtypes:
             raise ValueError(f"a cache is fp32, fp16 or bf16, not {k.dtype}")
         # the stride of a dimension of one entry is never used
         strides = [0 if n == 1 else s for n, s in zip(k.shape, k.stride())]
@@ -327,56 +348,61 @@ class KvCache:
         self.k, self.v = k, v
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.get_device()  # -1: host memory, which no kernel takes
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _KV_DTYPES[str(k.dtype)], self.layers, self.pages,
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _Torch.kv_dtypes[k.dtype], self.layers, self.pages,
                                 self.page_size, self.kv_heads, self.head_dim, *strides[:4])
         self.ref = ctypes.byref(self.desc)
 
 
-def _on_device(device: int, stream, call, what: str) -> None:
-    """call(stream) with `device` current, on `stream` or that device's current one."""
-    import torch
-
+def _launch(device: int, stream, what: str, call, *args) -> None:
+    """call(*args, stream) with `device` current, on `stream` or that device's current one."""
     if device < 0:
         raise ValueError("expected a CUDA tensor (device memory)")
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
-    handle = stream if isinstance(stream, int) else stream.cuda_stream
-    if torch.cuda.current_device() == device:
-        check(call(handle), what)
+    handle = _Torch.stream(device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+    if _Torch.device() == device:
+        check(call(*args, handle), what)
     else:
+        import torch
+
         with torch.cuda.device(device):
-            check(call(handle), what)
+            check(call(*args, handle), what)
 
 
 def _head_rows(t, name, rows, heads, dim, device):
     """(pointer, floats between rows) of an fp32 tensor [rows, heads, dim] whose rows are contiguous."""
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 3 or (rows is not None and shape[0] != rows) or shape[1] != heads or shape[2] != dim:
-        raise ValueError(f"{name}: expected [{'rows' if rows is None else rows}, {heads}, {dim}], got {list(shape)}")
-    if str(t.dtype) != "torch.float32" or t.get_device() != device:
+    if t.shape != (rows, heads, dim):
+        raise ValueError(f"{name}: expected [{rows}, {heads}, {dim}], got {list(t.shape)}")
+    if t.dtype is not _Torch.f32 or t.get_device() != device:
         raise ValueError(f"{name}: expected an fp32 tensor on the cache's device")
-    if (dim > 1 and strides[2] != 1) or (heads > 1 and strides[1] != dim):
+    row, head, one = t.stride()
+    if (one != 1 and dim > 1) or (head != dim and heads > 1):
         raise ValueError(f"{name}: expected contiguous heads within a row")
-    return t.data_ptr(), strides[0] if shape[0] > 1 else heads * dim
+    return t.data_ptr(), row if rows > 1 else heads * dim
 
 
 def _vector(t, name, n, dtype, device):
-    """Pointer of a contiguous 1-D tensor of n entries (None: no pointer)."""
+    """Pointer of a contiguous 1-D tensor of n entries (None: 0)."""
     if t is None:
-        return None
-    if t.dim() != 1 or t.numel() != n or str(t.dtype) != dtype or t.get_device() != device or not t.is_contiguous():
+        return 0
+    if t.shape != (n,) or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {n} entries on the cache's device")
     return t.data_ptr()
 
 
 def _table(t, device):
     """(pointer, rows, columns, ints between rows) of a page table [sequences, pages]."""
-    if t.dim() != 2 or str(t.dtype) != "torch.int32" or t.get_device() != device:
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not _Torch.i32 or t.get_device() != device:
         raise ValueError("page_table: expected an int32 tensor [sequences, pages] on the cache's device")
-    (rows, cols), strides = t.shape, t.stride()
-    if cols > 1 and strides[1] != 1:
+    (rows, cols), (row, one) = shape, t.stride()
+    if one != 1 and cols > 1:
         raise ValueError("page_table: expected contiguous rows")
-    return t.data_ptr(), rows, cols, strides[0] if rows > 1 else cols
+    return t.data_ptr(), rows, cols, row if rows > 1 else cols
+
+
+def _rows_and_heads(q):
+    if len(q.shape) != 3:
+        raise ValueError(f"q: expected [rows, heads, head_dim], got {list(q.shape)}")
+    return q.shape[:2]
 
 
 def rope_turns(rot_dim: int, theta: float = 500000.0, scaling: str = "none", factor: float = 1.0,
@@ -408,21 +434,20 @@ def rope_append(q_out, q, k, v, cache: KvCache, layer: int, pos, page_table, tur
     (negative: padding, skipped); seq int32 [m], the token's row of page_table
     (None: its own number).  turns: rope_turns (None: no rotation).
     """
-    d, device = cache.head_dim, cache.device
-    m, heads = q.shape[0], q.shape[1]
-    q_ptr, q_stride = _head_rows(q, "q", None, heads, d, device)
-    o_ptr, o_stride = _head_rows(q_out, "q_out", m, heads, d, device)
-    k_ptr, k_stride = _head_rows(k, "k", m, cache.kv_heads, d, device)
-    v_ptr, v_stride = _head_rows(v, "v", m, cache.kv_heads, d, device)
+    d, device, kv_heads = cache.head_dim, cache.device, cache.kv_heads
+    m, heads = _rows_and_heads(q)
+    q_ptr, q_stride = _head_rows(q, "q", m, heads, d, device)
+    o_ptr, o_stride = (q_ptr, q_stride) if q_out is q else _head_rows(q_out, "q_out", m, heads, d, device)
+    k_ptr, k_stride = _head_rows(k, "k", m, kv_heads, d, device)
+    v_ptr, v_stride = _head_rows(v, "v", m, kv_heads, d, device)
     t_ptr, t_rows, t_cols, t_stride = _table(page_table, device)
     pairs = 0 if turns is None else turns.numel()
-    op = RopeOp(m, heads, 2 * pairs, int(interleaved), amplitude, eps,
-                _vector(turns, "turns", pairs, "torch.float64", device), o_ptr, q_ptr, k_ptr, v_ptr, o_stride,
-                q_stride, k_stride, v_stride, _vector(q_norm, "q_norm", d, "torch.float32", device),
-                _vector(k_norm, "k_norm", d, "torch.float32", device),
-                _vector(pos, "pos", m, "torch.int32", device), _vector(seq, "seq", m, "torch.int32", device),
-                t_ptr, t_rows, t_cols, t_stride)
-    _on_device(device, stream, lambda s: lib().mli_rope_append(op, cache.ref, layer, s), "rope_append")
+    op = RopeOp.from_buffer_copy(_ROPE_FIELDS.pack(
+        m, heads, 2 * pairs, interleaved, amplitude, eps, _vector(turns, "turns", pairs, _Torch.f64, device), o_ptr,
+        q_ptr, k_ptr, v_ptr, o_stride, q_stride, k_stride, v_stride, _vector(q_norm, "q_norm", d, _Torch.f32, device),
+        _vector(k_norm, "k_norm", d, _Torch.f32, device), _vector(pos, "pos", m, _Torch.i32, device),
+        _vector(seq, "seq", m, _Torch.i32, device), t_ptr, t_rows, t_cols, t_stride))
+    _launch(device, stream, "rope_append", lib().mli_rope_append, op, cache.ref, layer)
 
 
 def paged_attention_workspace(cache: KvCache, rows: int, heads: int):
@@ -446,23 +471,22 @@ def paged_attention(out, q, cache: KvCache, layer: int, page_table, lengths, sca
     paged_attention_workspace; calls that share one must not overlap.
     """
     d, device = cache.head_dim, cache.device
-    rows, heads = q.shape[0], q.shape[1]
-    q_ptr, q_stride = _head_rows(q, "q", None, heads, d, device)
+    rows, heads = _rows_and_heads(q)
+    q_ptr, q_stride = _head_rows(q, "q", rows, heads, d, device)
     o_ptr, o_stride = _head_rows(out, "out", rows, heads, d, device)
     t_ptr, t_rows, t_cols, t_stride = _table(page_table, device)
-    op = AttentionOp(rows, heads, scale, o_ptr, q_ptr, o_stride, q_stride,
-                     _vector(lengths, "lengths", rows, "torch.int32", device),
-                     _vector(seq, "seq", rows, "torch.int32", device), t_ptr, t_rows, t_cols, t_stride,
-                     _vector(workspace, "workspace", workspace.numel(), "torch.uint8", device), workspace.numel())
-    _on_device(device, stream, lambda s: lib().mli_paged_attention(op, cache.ref, layer, s), "paged_attention")
+    w_bytes = workspace.numel()
+    op = AttentionOp.from_buffer_copy(_ATTENTION_FIELDS.pack(
+        rows, heads, scale, o_ptr, q_ptr, o_stride, q_stride, _vector(lengths, "lengths", rows, _Torch.i32, device),
+        _vector(seq, "seq", rows, _Torch.i32, device), t_ptr, t_rows, t_cols, t_stride,
+        _vector(workspace, "workspace", w_bytes, _Torch.u8, device), w_bytes))
+    _launch(device, stream, "paged_attention", lib().mli_paged_attention, op, cache.ref, layer)
 
 
 def kv_copy_pages(cache: KvCache, src, dst, stream=None):
     """Copies pages src[i] to dst[i] (int32 tensors) in every layer of a cache,
     keys and values; pairs with a negative entry are skipped.  No dst may be
     another pair's src or dst."""
-    n = src.numel()
-    s_ptr = _vector(src, "src", n, "torch.int32", cache.device)
-    d_ptr = _vector(dst, "dst", n, "torch.int32", cache.device)
-    _on_device(cache.device, stream, lambda s: lib().mli_kv_copy_pages(cache.ref, s_ptr, d_ptr, n, s),
-               "kv_copy_pages")
+    n, device = src.numel(), cache.device
+    _launch(device, stream, "kv_copy_pages", lib().mli_kv_copy_pages, cache.ref,
+            _vector(src, "src", n, _Torch.i32, device), _vector(dst, "dst", n, _Torch.i32, device), n)
