@@ -12,9 +12,10 @@
 namespace mli {
 namespace {
 
-constexpr int kAppendWarps = 4;
+// Two warps: each repeats a token's set-up, so 8192 tokens of 24 / 8 heads of 128 took 57 us with four; with one (52 us)
+// 1999 tokens of 35 / 5 heads of 80 took 31 us instead of 22.
+constexpr int kAppendWarps = 2;
 constexpr int kAppendThreads = kAppendWarps * 32;
-constexpr int kBatch = 4;  // heads whose values a lane holds at once
 
 // Where the other value of a rotated pair comes from.
 enum Partner {
@@ -33,51 +34,51 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
 }
 
-// A pass over memory: a token's heads are read once, 16 bytes a lane, and written once.  2^shift lanes hold a head,
+// A pass over memory: a token's heads are read once, 16 bytes a lane, and written once.  kLanes lanes hold a head,
 // kQuads times four values each; a warp's heads go in batches whose reads are all under way while the CTA computes
 // its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
 // values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
-template <typename T, int kQuads>
-__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c,
-                                                                     int shift, Partner partner) {
+template <typename T, int kLanes, int kQuads, Partner kPartner>
+__global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
   __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
   griddep_wait();
   griddep_launch_dependents();
   const int t = blockIdx.x;
   const int pos = op.pos[t];
   if (pos < 0) return;  // padding
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int lanes = 1 << shift, l = lane & (lanes - 1), sub = lane >> shift;
-  const int dim = c.head_dim, half = op.rot_dim / 2, total = op.heads + 2 * c.kv_heads;
-  const int at_once = 32 >> shift, step = gridDim.y * kAppendWarps * at_once;
-
+  constexpr int kAtOnce = 32 / kLanes, kBatch = 4 / kQuads;  // heads of a warp side by side, and after one another
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int l = lane % kLanes, sub = lane / kLanes;
+  const int dim = c.head_dim, half = op.rot_dim / 2, keys = op.heads, values = op.heads + c.kv_heads;
+  const int total = values + c.kv_heads, step = gridDim.y * kAppendWarps * kAtOnce;
+  // value 0 of a head, were the keys' and values' heads counted on from the queries'
+  const float* const q_row = op.q + t * op.q_stride;
+  const float* const k_row = op.k + (t * op.k_stride - static_cast<long long>(keys) * dim);
+  const float* const v_row = op.v + (t * op.v_stride - static_cast<long long>(values) * dim);
   const auto source = [&](int h) {
-    return h < op.heads                ? op.q + t * op.q_stride + static_cast<long long>(h) * dim
-           : h < op.heads + c.kv_heads ? op.k + t * op.k_stride + static_cast<long long>(h - op.heads) * dim
-                                       : op.v + t * op.v_stride + static_cast<long long>(h - op.heads - c.kv_heads) * dim;
+    return (h < keys ? q_row : h < values ? k_row : v_row) + static_cast<long long>(h) * dim;
   };
   float4 x[kBatch][kQuads];
   const auto read = [&](int first) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = first + b * step + sub;
+      const float* p = source(h) + 4 * l;
 #pragma unroll
-      for (int i = 0; i < kQuads; ++i) {
-        const int e = 4 * (l + 32 * i);
-        x[b][i] = h < total && e < dim ? *reinterpret_cast<const float4*>(source(h) + e)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      for (int i = 0; i < kQuads; ++i)
+        x[b][i] = h < total && 4 * (l + 32 * i) < dim ? *reinterpret_cast<const float4*>(p + 128 * i)
+                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  int first = (blockIdx.y * kAppendWarps + warp) * at_once;
+  int first = (blockIdx.y * kAppendWarps + warp) * kAtOnce;
   read(first);
 
   // the token's slot, or -1
   long long slot = -1;
-  const int seq = op.seq ? op.seq[t] : t;
-  if (seq >= 0 && seq < op.table_rows && pos / c.page_size < op.table_cols) {
-    const int page = op.page_table[seq * op.table_stride + pos / c.page_size];
-    if (page >= 0 && page < c.pages) slot = page * c.page_stride + (pos % c.page_size) * c.slot_stride;
+  const int seq = op.seq ? op.seq[t] : t, col = pos / c.page_size;
+  if (seq >= 0 && seq < op.table_rows && col < op.table_cols) {
+    const int page = op.page_table[seq * op.table_stride + col];
+    if (page >= 0 && page < c.pages) slot = page * c.page_stride + (pos - col * c.page_size) * c.slot_stride;
   }
   if (slot < 0 && threadIdx.x == 0 && blockIdx.y == 0) record_device_error(kDevPageRange);
 
@@ -98,75 +99,87 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const mli_r
     for (int j = 0; j < 4; ++j) {
       const int e = 4 * (l + 32 * i) + j;
       const bool on = e < op.rot_dim;
-      const bool second = op.interleaved ? (e & 1) : e >= half;
-      const int pair = !on ? 0 : op.interleaved ? e >> 1 : second ? e - half : e;
+      const bool second = kPartner == kSameQuad ? (j & 1) : e >= half;
+      const int pair = !on ? 0 : kPartner == kSameQuad ? e >> 1 : second ? e - half : e;
       cs[i][j] = on ? s_cos[pair] : 1.f;
       sn[i][j] = on ? (second ? s_sin[pair] : -s_sin[pair]) : 0.f;
     }
+  const bool norms = op.q_norm || op.k_norm;
+  const float per_dim = 1.f / dim;
+  float* const q_to = op.q_out + t * op.q_out_stride + 4 * l;
+  T* const k_to = c.k + slot + 4 * l;
+  T* const v_to = c.v + slot + 4 * l;
 
-  while (first < total) {
+  for (; first < total; first += kBatch * step, read(first)) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = first + b * step + sub;
-      const bool is_v = h >= op.heads + c.kv_heads;
-      const float* w = h < op.heads ? op.q_norm : is_v ? nullptr : op.k_norm;
+      float y[kQuads][4];
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        y[i][0] = x[b][i].x;
+        y[i][1] = x[b][i].y;
+        y[i][2] = x[b][i].z;
+        y[i][3] = x[b][i].w;
+      }
+      const float* w = h < keys ? op.q_norm : h < values ? op.k_norm : nullptr;
       float inv = 1.f;
-      if (op.q_norm || op.k_norm) {
+      if (norms) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
-          ss += (x[b][i].x * x[b][i].x + x[b][i].y * x[b][i].y) + (x[b][i].z * x[b][i].z + x[b][i].w * x[b][i].w);
-        for (int off = lanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        if (w) inv = 1.f / sqrtf(ss / dim + op.eps);
-      }
-      float y[kQuads][4], other[kQuads][4];
+          ss += (y[i][0] * y[i][0] + y[i][1] * y[i][1]) + (y[i][2] * y[i][2] + y[i][3] * y[i][3]);
 #pragma unroll
-      for (int i = 0; i < kQuads; ++i) {
-        const int e = 4 * (l + 32 * i);
-        const float4 u = w && e < dim ? *reinterpret_cast<const float4*>(w + e) : make_float4(1.f, 1.f, 1.f, 1.f);
-        y[i][0] = x[b][i].x * inv * u.x;
-        y[i][1] = x[b][i].y * inv * u.y;
-        y[i][2] = x[b][i].z * inv * u.z;
-        y[i][3] = x[b][i].w * inv * u.w;
+        for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (w) inv = rsqrtf(ss * per_dim + op.eps);
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+          const int e = 4 * (l + 32 * i);
+          const float4 u = w && e < dim ? *reinterpret_cast<const float4*>(w + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+          y[i][0] *= inv * u.x;
+          y[i][1] *= inv * u.y;
+          y[i][2] *= inv * u.z;
+          y[i][3] *= inv * u.w;
+        }
       }
+      float z[kQuads][4];
 #pragma unroll
       for (int i = 0; i < kQuads; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int e = 4 * (l + 32 * i) + j;
-          if (partner == kSameQuad) {
-            other[i][j] = y[i][j ^ 1];
-          } else if (kQuads == 1 && partner == kOtherLane) {
-            other[i][j] = __shfl_sync(0xffffffffu, y[i][j], l < half / 4 ? l + half / 4 : l - half / 4, lanes);
-          } else if (kQuads == 2 && partner == kOtherQuad) {
-            other[i][j] = y[i ^ 1][j];
+          float other;
+          if constexpr (kPartner == kSameQuad) {
+            other = y[i][j ^ 1];
+          } else if constexpr (kPartner == kOtherLane) {
+            other = __shfl_sync(0xffffffffu, y[i][j], l < half / 4 ? l + half / 4 : l - half / 4, kLanes);
+          } else if constexpr (kPartner == kOtherQuad) {
+            other = y[i ^ 1][j];
           } else {
             const int o = e < half ? e + half : e - half;
-            other[i][j] = h < total && !is_v && e < op.rot_dim ? source(h)[o] * inv * (w ? w[o] : 1.f) : 0.f;
+            other = h < values && e < op.rot_dim ? source(h)[o] * (inv * (w ? w[o] : 1.f)) : 0.f;
           }
-          if (e >= op.rot_dim) other[i][j] = 0.f;
+          // behind rot_dim the other value, whatever it is, is not part of the result
+          z[i][j] = h >= values ? y[i][j] : fmaf(y[i][j], cs[i][j], (e < op.rot_dim ? other : 0.f) * sn[i][j]);
         }
-      __syncwarp();  // q_out may be q, whose values a neighbour reads again
-      if (h < total && (h < op.heads || slot >= 0)) {
+      if (kPartner == kReload) __syncwarp();  // q_out may be q, whose values a neighbour reads again
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-          const int e = 4 * (l + 32 * i);
-          if (e >= dim) continue;
-          float z[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[j] = is_v ? y[i][j] : fmaf(y[i][j], cs[i][j], other[i][j] * sn[i][j]);
-          if (h < op.heads)
-            store4(op.q_out + t * op.q_out_stride + static_cast<long long>(h) * dim + e, z);
-          else if (!is_v)
-            store4(c.k + slot + (h - op.heads) * c.head_stride + e, z);
-          else
-            store4(c.v + slot + (h - op.heads - c.kv_heads) * c.head_stride + e, z);
-        }
+      for (int i = 0; i < kQuads; ++i) {
+        if (4 * (l + 32 * i) >= dim) continue;
+        if (h < keys)
+          store4(q_to + static_cast<long long>(h) * dim + 128 * i, z[i]);
+        else if (h < total && slot >= 0)
+          store4((h < values ? k_to + (h - keys) * c.head_stride : v_to + (h - values) * c.head_stride) + 128 * i, z[i]);
       }
     }
-    first += kBatch * step;
-    read(first);
   }
+}
+
+template <typename T, int kLanes, int kQuads>
+auto append_kernel(Partner partner) {
+  return partner == kSameQuad ? rope_append_kernel<T, kLanes, kQuads, kSameQuad>
+         : partner == kReload ? rope_append_kernel<T, kLanes, kQuads, kReload>
+                              : rope_append_kernel<T, kLanes, kQuads, kQuads == 2 ? kOtherQuad : kOtherLane>;
 }
 
 template <typename T>
@@ -174,21 +187,20 @@ int launch_append(const mli_rope_op& op, const mli_kv_cache& cache, int layer, c
   cudaError_t e = cudaSuccess;
   const DeviceInfo& dev = current_device(&e);
   if (e != cudaSuccess) return check_cuda(e);
-  int shift = 0;
-  while (shift < 5 && (4 << shift) < cache.head_dim) ++shift;
-  const int half = op.rot_dim / 2;
-  const bool wide = cache.head_dim > 128;
-  const Partner partner = op.interleaved || half == 0 ? kSameQuad
-                          : !wide && half % 4 == 0    ? kOtherLane
-                          : wide && half == 128       ? kOtherQuad
-                                                      : kReload;
+  const int half = op.rot_dim / 2, dim = cache.head_dim;
+  const Partner partner = op.interleaved || half == 0                       ? kSameQuad
+                          : dim > 128 ? (half == 128 ? kOtherQuad : kReload)
+                          : half % 4 == 0                                   ? kOtherLane
+                                                                            : kReload;
+  const auto kernel = dim <= 64    ? append_kernel<T, 16, 1>(partner)
+                      : dim <= 128 ? append_kernel<T, 32, 1>(partner)
+                                   : append_kernel<T, 32, 2>(partner);
   // few tokens: their heads over as many CTAs as give each warp one turn, or as fill the SMs four times
-  const int at_once = kAppendWarps * (32 >> shift), heads = op.heads + 2 * cache.kv_heads;
+  const int at_once = kAppendWarps * (dim <= 64 ? 2 : 1), heads = op.heads + 2 * cache.kv_heads;
   const int most = (heads + at_once - 1) / at_once, fill = 4 * dev.sm_count / op.m;
   const int share = fill < 1 ? 1 : fill < most ? fill : most;
   const dim3 grid(static_cast<unsigned>(op.m), static_cast<unsigned>(share));
-  return check_cuda(launch(wide ? rope_append_kernel<T, 2> : rope_append_kernel<T, 1>, grid, dim3(kAppendThreads), 0,
-                           stream, true, op, cache_layer<T>(cache, layer), shift, partner));
+  return check_cuda(launch(kernel, grid, dim3(kAppendThreads), 0, stream, true, op, cache_layer<T>(cache, layer)));
 }
 
 constexpr int kCopyThreads = 256;

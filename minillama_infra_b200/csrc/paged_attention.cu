@@ -94,11 +94,12 @@ struct Args {
   unsigned* arrivals;  // [rows * kv_heads * chunks], zero between calls
 };
 
-// A piece of a segment: the unnormalised output, the maximum, the sum and c of each head.
+// A piece of a segment: of each head the unnormalised output, the maximum, the sum and c.
 template <int kDim, int kHeads>
 struct Piece {
   float o[kHeads][kDim];
-  float m[kHeads], l[kHeads], c[kHeads], pad[kHeads];
+  float m[kHeads], l[kHeads], c[kHeads];
+  float weight[kHeads];  // beside the other pieces of its CTA
 };
 // What a piece of maximum m counts beside one of maximum top (no piece: 1, and its sums are zero).
 __device__ __forceinline__ float piece_weight(float m, float top, float c) {
@@ -190,6 +191,7 @@ struct TensorMath {
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kScratch = 0;
   static constexpr int kSteps = kUsed / 16;
+  static constexpr int kReadBytes = kUsed * 2;  // of a token
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;
   using Part = Piece<kDim, kHeads>;
 
@@ -386,6 +388,7 @@ struct FloatMath {
   static constexpr int kTok = kSlotBytes / (kDim * 4);  // 32, 16 or 8 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kScratch = kHeads * (kDim + kTok);  // floats: q, then the tile's p
+  static constexpr int kReadBytes = kDim * 4;  // of a token
   static constexpr int kParts = 32 / kTok;   // lanes of a token's score
   static constexpr int kChunks = kDim / 4;   // 16-byte pieces of a token
   static constexpr int kRows = kChunks < 32 ? 32 / kChunks : 1;  // tokens side by side in the outputs' sum
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   float* scratch = reinterpret_cast<float*>(first_pieces + kWarps) + warp * Math::kScratch;
   const int dim = cache.head_dim, items = cache.kv_heads * a.chunks;
   const int live_chunks = dim * static_cast<int>(sizeof(T)) / 16;
-  if (live_chunks < kChunks) {  // the columns that no token fills
+  if (live_chunks * 16 < Math::kReadBytes) {  // columns that are multiplied, but that no token fills
     for (int i = lane; i < kSlots * kSlotBytes / 16; i += 32)
       reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
@@ -839,7 +842,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   __syncthreads();
 
   // ---- the join -------------------------------------------------------------------
-  // Every warp lists the segments that the CTA holds pieces of: lane i looks at piece i, group g begins at the g-th
+  // Every warp lists the segments that the CTA holds pieces of: lane i looks at piece i, and a group begins at each
   // piece whose segment is not that of the piece before.
   Held held = Held{0, 0, 0, 0, 0};
   if (lane < 2 * kWarps) held = s_held[lane];
@@ -848,6 +851,21 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   const long long left = __shfl_sync(0xffffffffu, held.start, below ? 31 - __clz(below) : lane);
   const unsigned firsts = __ballot_sync(0xffffffffu, held.used != 0 && (below == 0 || left != held.start));
   const int groups = __popc(firsts);
+  const auto members_of = [&](int from) {  // of the group that begins at piece `from`
+    const unsigned later = firsts & ~((2u << from) - 1);
+    return used & ~((1u << from) - 1) & (later ? (later & -later) - 1 : ~0u);
+  };
+  // a thread a piece and head: what it weighs beside the others of its group
+  for (int i = tid; i < 2 * kWarps * Math::kHeads; i += kThreads) {
+    const int j = i / Math::kHeads, h = i % Math::kHeads;
+    if (!((used >> j) & 1)) continue;
+    const unsigned members = members_of(31 - __clz(firsts & ((2u << j) - 1)));
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2 * kWarps; ++k) top = fmaxf(top, (members >> k) & 1 ? piece_at(k)->m[h] : -INFINITY);
+    piece_at(j)->weight[h] = piece_weight(piece_at(j)->m[h], top, piece_at(j)->c[h]);
+  }
+  __syncthreads();
   const auto group_lane = [&](int g) {
     unsigned rest = firsts;
     for (; g > 0; --g) rest &= rest - 1;
@@ -865,22 +883,15 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   for (int i = tid; i < groups * kItems; i += kThreads) {
     const int from = group_lane(i / kItems);
     const Held g = group_held(from);
-    const unsigned later = firsts & ~((2u << from) - 1);
-    const unsigned members = used & ~((1u << from) - 1) & (later ? (later & -later) - 1 : ~0u);
+    const unsigned members = members_of(from);
     const int h = i % kItems / kQuads, e = 4 * (i % kQuads);
     if (h >= heads_of(g.item)) continue;
-    // all pieces' reads at once, those of others left out
-    float m[2 * kWarps], top = -INFINITY, sum_l = 0.f;
-    const float c = piece_at(from)->c[h];
-#pragma unroll
-    for (int j = 0; j < 2 * kWarps; ++j) m[j] = (members >> j) & 1 ? piece_at(j)->m[h] : -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 2 * kWarps; ++j) top = fmaxf(top, m[j]);
+    float sum_l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 2 * kWarps; ++j)
       if ((members >> j) & 1) {
-        const float w = piece_weight(m[j], top, c);
+        const float w = piece_at(j)->weight[h];
         const float4 v = *reinterpret_cast<const float4*>(&piece_at(j)->o[h][e]);
         sum_l = fmaf(w, piece_at(j)->l[h], sum_l);
         y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
@@ -894,9 +905,11 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       Part* to = parts + 2 * cta + (g.start > cta_begin ? 1 : 0);
       *reinterpret_cast<float4*>(&to->o[h][e]) = y;
       if (e == 0) {
+        float top = -INFINITY;
+        for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
         to->m[h] = top;
         to->l[h] = sum_l;
-        to->c[h] = c;
+        to->c[h] = piece_at(from)->c[h];
       }
     }
   }
@@ -907,12 +920,18 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   const Held ends[2] = {end_group(0), end_group(1)};
   const bool shared[2] = {groups > 0 && beyond(ends[0]), groups > 1 && beyond(ends[1])};
   if (!shared[0] && !shared[1]) return;
+  int first_ctas[2], counts[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    first_ctas[k] = shared[k] ? shares.owner(ends[k].start) : 0;
+    counts[k] = shared[k] ? shares.owner(ends[k].start + ends[k].tiles - 1) - first_ctas[k] + 1 : 0;
+  }
   __syncthreads();
   if (tid < 2) {
     const Held g = tid == 0 ? ends[0] : ends[1];
     bool last = false;
     if (tid == 0 ? shared[0] : shared[1]) {
-      const unsigned most = shares.owner(g.start + g.tiles - 1) - shares.owner(g.start);
+      const unsigned most = (tid == 0 ? counts[0] : counts[1]) - 1;
       // wraps to zero at the last arrival: ready for the next call
       last = arrive(a.arrivals + static_cast<long long>(g.row) * items + g.item, most) == most;
     }
@@ -923,14 +942,14 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const int k = i / kItems, h = i % kItems / kQuads, e = 4 * (i % kQuads);
     const Held& g = k == 0 ? ends[0] : ends[1];
     if (!s_last[k] || h >= heads_of(g.item) || e >= dim) continue;
-    const int first_cta = shares.owner(g.start), count = shares.owner(g.start + g.tiles - 1) - first_cta + 1;
+    const int first_cta = k == 0 ? first_ctas[0] : first_ctas[1], count = k == 0 ? counts[0] : counts[1];
     // slot 0 of all CTAs but the first, in which the segment may be the last one
     const Part* other = parts + 2 * first_cta;
     const Part* first_part = other + (g.start > shares.begin(first_cta) ? 1 : 0);
     const float c = __ldcg(&first_part->c[h]);
     float top = -INFINITY, sum_l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 4;  // parts read at once
+    constexpr int kBatch = 8;  // parts read at once
     for (int j0 = 0; j0 < count; j0 += kBatch) {
       float m[kBatch], l[kBatch];
       float4 v[kBatch];
