@@ -51,12 +51,22 @@ __device__ __forceinline__ unsigned divide(unsigned n, const FastDiv& d) {
   return static_cast<unsigned>((static_cast<unsigned long long>(n) * d.mul) >> d.shift);
 }
 
-__device__ __forceinline__ void cp_async16(unsigned smem, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
+// Keys and values pass through L2 once a step: marked to be evicted first, they leave the page table, the queries,
+// the partial results and the kernel's own code there.
+__device__ __forceinline__ unsigned long long stream_policy() {
+  unsigned long long p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp_async16(unsigned smem, const void* src, unsigned long long policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "l"(policy)
+               : "memory");
 }
 // The same where `live`, else zeros, the source not read.
-__device__ __forceinline__ void cp_async16(unsigned smem, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(unsigned smem, const void* src, unsigned long long policy, bool live) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(smem), "l"(src),
+               "r"(live ? 16 : 0), "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -744,6 +754,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     constexpr int kAtOnce = kChunks < 32 ? 32 / kChunks : 1, kWide = kChunks > 32 ? kChunks / 32 : 1;
     const int sub = kChunks < 32 ? lane / kChunks : 0, chunk = lane % kChunks;
     const unsigned lane_to = sub * kRowBytes + (((chunk & 7) ^ sub) << 4) + ((chunk >> 3) << 7);
+    const unsigned long long policy = stream_policy();
     const auto fill = [&](int slot, const T* from) {
       const unsigned to = smem_u32(ring) + slot * kSlotBytes + lane_to;
       const char* src = reinterpret_cast<const char*>(from) + chunk * 16;
@@ -756,9 +767,9 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
           for (int j = 0; j < kWide; ++j) {
             if (chunk + 32 * j >= live_chunks) continue;
             if constexpr (decltype(whole)::value)
-              cp_async16(p + 512 * j, src + at + 512 * j);
+              cp_async16(p + 512 * j, src + at + 512 * j, policy);
             else
-              cp_async16(p + 512 * j, src + (at >= 0 ? at : 0) + 512 * j, at >= 0);
+              cp_async16(p + 512 * j, src + (at >= 0 ? at : 0) + 512 * j, policy, at >= 0);
           }
         }
       };
