@@ -153,12 +153,12 @@ __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, uns
                                     unsigned b1, bool fresh) {
   const float c[4] = {fresh ? 0.f : d[0], fresh ? 0.f : d[1], fresh ? 0.f : d[2], fresh ? 0.f : d[3]};
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
@@ -179,14 +179,12 @@ __device__ __forceinline__ void split3(float x, float y, unsigned& hi, unsigned&
 __device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], unsigned addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldmatrix4_trans(unsigned (&r)[4], unsigned addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 // Shared address of chunk `chunk ^ row & 7` given that of chunk `x` of the same row, x < 8 (rows begin on 128 bytes).
 __device__ __forceinline__ unsigned swizzled(unsigned first, int chunk) {
@@ -199,47 +197,51 @@ template <typename T, int kDim, int kUsed, bool kFew>
 struct TensorMath {
   static constexpr int kTok = kSlotBytes / (kDim * 2);  // 64, 32 or 16 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
-  static constexpr int kScratch = 0;
   static constexpr int kSteps = kUsed / 16;
+  // the third parts of 8 heads of 256 queries would not fit in registers beside the rest: they are in shared memory
+  static constexpr bool kThirdShared = kDim == 256 && !kFew;
+  static constexpr int kScratch = kThirdShared ? kSteps * 64 : 0;
   static constexpr int kReadBytes = kUsed * 2;  // of a token
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;
   using Part = Piece<kDim, kHeads>;
 
-  unsigned q[kSteps][kFew ? 4 : 6];
+  unsigned q[kSteps][kFew || kThirdShared ? 4 : 6];
   unsigned p[kTok / 8][kFew ? 2 : 3];
   float2 o[kUsed / 8];
   float m, l, c, keep;
   int head;  // this lane's head within the pass
   bool third;
 
-  // A pass begins: its queries, asked for here and taken apart in begin().
-  struct Queries {
-    float2 x[kSteps][2];
-  };
-  __device__ __forceinline__ void ask(Queries& raw, const float* qp, int heads, int dim) {
+  // A pass begins: its queries are read and taken apart.
+  __device__ __forceinline__ void begin(const float* qp, int heads, int dim, float scale, float* scratch) {
     const int lane = threadIdx.x & 31, g = lane >> 2, col = 2 * (lane & 3);
     head = kFew ? g & 3 : g;
     third = kFew && g >= 4;
     const float* row = qp + head * dim;
     const bool live = head < heads;
+    constexpr int kBatch = kSteps < 8 ? kSteps : 8;  // steps whose reads are under way at once
+    float2 x[kBatch][2];
+    const auto read = [&](int k0) {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int e = 16 * k + 8 * j + col;
-        raw.x[k][j] = live && e < dim ? *reinterpret_cast<const float2*>(row + e) : make_float2(0.f, 0.f);
-      }
-  }
-  __device__ __forceinline__ void begin(const Queries& raw, float scale, float*) {
+        for (int j = 0; j < 2; ++j) {
+          const int e = 16 * (k0 + k) + 8 * j + col;
+          x[k][j] = live && e < dim ? *reinterpret_cast<const float2*>(row + e) : make_float2(0.f, 0.f);
+        }
+    };
     c = scale;
     float up = 1.f;
-    const auto& x = raw.x;
     if (kUp != 1.f) {
       float top = 0.f;
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+      for (int k0 = kSteps - kBatch; k0 >= 0; k0 -= kBatch) {
+        read(k0);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int exponent = (__float_as_int(top) >> 23) & 255;
@@ -248,15 +250,22 @@ struct TensorMath {
       c = fmaxf(c * __int_as_float((254 - f) << 23), FLT_MIN);  // c = 0 would make c s of -inf a NaN
     }
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
+    for (int k0 = 0; k0 < kSteps; k0 += kBatch) {
+      if (k0 > 0 || kUp == 1.f) read(k0);  // the maximum's last batch is the first
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        unsigned hi, mid, lo;
-        split3<T>(x[k][j].x * up, x[k][j].y * up, hi, mid, lo);
-        q[k][2 * j] = third ? 0u : hi;
-        q[k][2 * j + 1] = third ? lo : mid;
-        if (!kFew) q[k][4 + j] = lo;
-      }
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          unsigned hi, mid, lo;
+          split3<T>(x[k][j].x * up, x[k][j].y * up, hi, mid, lo);
+          q[k0 + k][2 * j] = third ? 0u : hi;
+          q[k0 + k][2 * j + 1] = third ? lo : mid;
+          if constexpr (kThirdShared)
+            reinterpret_cast<unsigned*>(scratch)[(k0 + k) * 64 + 2 * lane + j] = lo;
+          else if constexpr (!kFew)
+            q[k0 + k][4 + j] = lo;
+        }
+    }
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
@@ -264,7 +273,7 @@ struct TensorMath {
   }
 
   // The tile's weights from its keys.  live: bit t for token t.
-  __device__ __forceinline__ void scores(unsigned keys, unsigned long long live, float*) {
+  __device__ __forceinline__ void scores(unsigned keys, unsigned long long live, const float* scratch) {
     const int lane = threadIdx.x & 31, mat = lane >> 3, in = lane & 7;
     float s[kTok / 8][4];
     // matrices (tokens 0-7, 8-15) x (dims 0-7, 8-15) of a 16-token block
@@ -272,6 +281,11 @@ struct TensorMath {
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const unsigned at = swizzled(row, 2 * k);
+      uint2 third_part = make_uint2(0u, 0u);
+      if constexpr (kThirdShared)
+        third_part = reinterpret_cast<const uint2*>(scratch)[k * 32 + lane];
+      else if constexpr (!kFew)
+        third_part = make_uint2(q[k][4], q[k][5]);
 #pragma unroll
       for (int n = 0; n < kTok / 16; ++n) {
         unsigned b[4];
@@ -280,7 +294,7 @@ struct TensorMath {
         for (int h = 0; h < 2; ++h) {
           float(&d)[4] = s[2 * n + h];
           mma<T>(d, q[k][0], q[k][1], q[k][2], q[k][3], b[2 * h], b[2 * h + 1], k == 0);
-          if (!kFew) mma<T>(d, q[k][4], 0u, q[k][5], 0u, b[2 * h], b[2 * h + 1], false);
+          if (!kFew) mma<T>(d, third_part.x, 0u, third_part.y, 0u, b[2 * h], b[2 * h + 1], false);
         }
       }
     }
@@ -323,7 +337,7 @@ struct TensorMath {
 
   // The tile's outputs from its values.  A tile's sum starts from zero, so that the tensor cores' accumulation
   // (which truncates) never runs over more than a tile.
-  __device__ __forceinline__ void outputs(unsigned values, float*) {
+  __device__ __forceinline__ void outputs(unsigned values, const float*) {
     const int lane = threadIdx.x & 31, mat = lane >> 3, in = lane & 7;
     const unsigned row = values + ((mat & 1) * 8 + in) * (kDim * 2) + (((mat >> 1) ^ in) << 4);
     const float2 keep2 = make_float2(keep, keep);
@@ -386,9 +400,8 @@ struct TensorMath {
 
 // ---- the products in fp32, fp32 caches ----------------------------------------
 //
-// A lane takes one token of the tile (or a part of its dims) for the scores
-// and four dims of a token (or eight) for the outputs; q and p come from shared memory
-// as broadcasts.
+// A lane takes a part of the dims of two tokens for the scores and four dims of a token
+// (or eight) for the outputs; q and p come from shared memory as broadcasts.
 __device__ __forceinline__ const float4* shared_float4(unsigned addr) {
   return reinterpret_cast<const float4*>(__cvta_shared_to_generic(addr));
 }
@@ -399,7 +412,8 @@ struct FloatMath {
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kScratch = kHeads * (kDim + kTok);  // floats: q, then the tile's p
   static constexpr int kReadBytes = kDim * 4;  // of a token
-  static constexpr int kParts = 32 / kTok;   // lanes of a token's score
+  static constexpr int kLanes = kTok / 2;    // side by side in the scores, two tokens each
+  static constexpr int kParts = 32 / kLanes;  // lanes that share a token's dims
   static constexpr int kChunks = kDim / 4;   // 16-byte pieces of a token
   static constexpr int kRows = kChunks < 32 ? 32 / kChunks : 1;  // tokens side by side in the outputs' sum
   static constexpr int kOwn = kChunks < 32 ? 1 : kChunks / 32;   // pieces of a token a lane sums
@@ -409,22 +423,15 @@ struct FloatMath {
   float2 o[kHeads][kOwn][2];
   float m[kHeads], l[kHeads], keep[kHeads], c;
 
-  struct Queries {
-    float4 x[kHeads * kChunks / 32];
-  };
-  __device__ __forceinline__ void ask(Queries& raw, const float* qp, int heads, int dim) {
+  __device__ __forceinline__ void begin(const float* qp, int heads, int dim, float scale, float* scratch) {
+    __syncwarp();
 #pragma unroll
     for (int k = 0; k < kHeads * kChunks / 32; ++k) {
       const int i = (threadIdx.x & 31) + 32 * k, h = i / kChunks, e = 4 * (i % kChunks);
-      raw.x[k] = h < heads && e < dim ? *reinterpret_cast<const float4*>(qp + h * dim + e)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+      reinterpret_cast<float4*>(scratch)[i] = h < heads && e < dim
+                                                  ? *reinterpret_cast<const float4*>(qp + h * dim + e)
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-  }
-  __device__ __forceinline__ void begin(const Queries& raw, float scale, float* scratch) {
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < kHeads * kChunks / 32; ++k)
-      reinterpret_cast<float4*>(scratch)[(threadIdx.x & 31) + 32 * k] = raw.x[k];
     __syncwarp();
     c = scale;
 #pragma unroll
@@ -440,39 +447,56 @@ struct FloatMath {
     const int lane = threadIdx.x & 31;
     const float4* keys = shared_float4(slot);
     const float4* qs = reinterpret_cast<const float4*>(scratch);
-    float* ps = scratch + kHeads * kDim;  // [kTok][kHeads]
-    const int t = lane % kTok, part = lane / kTok;
-    float2 acc[kHeads][2];
+    float4* ps = reinterpret_cast<float4*>(scratch + kHeads * kDim);  // [kTok][kHeads]
+    const int t = lane % kLanes, part = lane / kLanes;
+    float2 acc[2][kHeads][2];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) acc[h][0] = acc[h][1] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int k = part; k < kChunks; k += kParts) {
-      const float4 x = keys[t * kChunks + (k ^ (t & 7))];
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) acc[r][h][0] = acc[r][h][1] = make_float2(0.f, 0.f);
+    // of 8 neighbouring lanes with 4 tokens the two parts read pieces 4 apart: other banks
+    const int first = kLanes < 8 ? (part & 1) * 4 + (part >> 1) : part;
+#pragma unroll 2
+    for (int k = first; k < kChunks; k += kParts) {
+      const float4 x0 = keys[t * kChunks + (k ^ (t & 7))];
+      const float4 x1 = keys[(t + kLanes) * kChunks + (k ^ ((t + kLanes) & 7))];
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
         const float4 y = qs[h * kChunks + k];
-        acc[h][0] = fma2(make_float2(x.x, x.y), make_float2(y.x, y.y), acc[h][0]);
-        acc[h][1] = fma2(make_float2(x.z, x.w), make_float2(y.z, y.w), acc[h][1]);
+        acc[0][h][0] = fma2(make_float2(x0.x, x0.y), make_float2(y.x, y.y), acc[0][h][0]);
+        acc[0][h][1] = fma2(make_float2(x0.z, x0.w), make_float2(y.z, y.w), acc[0][h][1]);
+        acc[1][h][0] = fma2(make_float2(x1.x, x1.y), make_float2(y.x, y.y), acc[1][h][0]);
+        acc[1][h][1] = fma2(make_float2(x1.z, x1.w), make_float2(y.z, y.w), acc[1][h][1]);
       }
     }
-    const bool on = (live >> t) & 1;
+    float p[2][kHeads];
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      float s = (acc[h][0].x + acc[h][0].y) + (acc[h][1].x + acc[h][1].y);
 #pragma unroll
-      for (int off = kTok; off < 32; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
-      s = on ? s : -INFINITY;
-      float top = s;
+      for (int r = 0; r < 2; ++r) {
+        float s = (acc[r][h][0].x + acc[r][h][0].y) + (acc[r][h][1].x + acc[r][h][1].y);
 #pragma unroll
-      for (int off = kTok / 2; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        for (int off = kLanes; off < 32; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
+        p[r][h] = (live >> (t + r * kLanes)) & 1 ? s : -INFINITY;
+      }
+      float top = fmaxf(p[0][h], p[1][h]);
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       top = fmaxf(top, m[h]);
       const float base = top == -INFINITY ? 0.f : top;
       keep[h] = exp2_approx((m[h] - base) * c);
       m[h] = top;
-      const float p = exp2_approx((s - base) * c);
-      l[h] = fmaf(l[h], keep[h], part == 0 ? p : 0.f);
-      if (part == 0) ps[t * kHeads + h] = p;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) p[r][h] = exp2_approx((p[r][h] - base) * c);
+      l[h] = fmaf(l[h], keep[h], part == 0 ? p[0][h] + p[1][h] : 0.f);
     }
+    if (part == 0)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int h4 = 0; h4 < kHeads / 4; ++h4)
+          ps[(t + r * kLanes) * (kHeads / 4) + h4] =
+              make_float4(p[r][4 * h4], p[r][4 * h4 + 1], p[r][4 * h4 + 2], p[r][4 * h4 + 3]);
     __syncwarp();
   }
 
@@ -570,35 +594,32 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
   if (seq < 0 || seq >= a.table_rows) return Row{0, 0, true};
   return Row{len > a.room ? static_cast<int>(a.room) : len, seq, len > a.room};
 }
-__device__ __forceinline__ long long quotient(long long n, long long by) {  // of numbers >= 0
-  return ((n | by) >> 32) == 0 ? static_cast<unsigned>(n) / static_cast<unsigned>(by) : n / by;
-}
 
 // A segment's place among all tiles.
 struct Segment {
-  long long start;  // first tile
-  int row, item;    // item: key-value head * chunks + chunk
+  int start;      // first tile
+  int row, item;  // item: key-value head * chunks + chunk
   int seq, tiles, tokens;
 };
 
-// All tiles in equal shares: the first `more` of `among` take one more than the others.
+// Tiles [first, to) in equal shares: the first `more` of `among` take one more than the others.
 struct Shares {
-  long long first, each, more;
-  __device__ __forceinline__ Shares(long long from, long long to, int among) : first(from) {
-    each = quotient(to - from, among);
+  int first, each, more;
+  __device__ __forceinline__ Shares(int from, int to, int among) : first(from) {
+    each = (to - from) / among;
     more = to - from - each * among;
   }
-  __device__ __forceinline__ long long begin(int i) const { return first + i * each + (i < more ? i : more); }
-  __device__ __forceinline__ int owner(long long tile) const {
-    const long long longer = more * (each + 1);
+  __device__ __forceinline__ int begin(int i) const { return first + i * each + min(i, more); }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int longer = more * (each + 1);
     tile -= first;
-    return static_cast<int>(tile < longer ? quotient(tile, each + 1) : more + quotient(tile - longer, each));
+    return tile < longer ? tile / (each + 1) : more + (tile - longer) / each;
   }
 };
 
 // A piece that a CTA holds in shared memory.
 struct Held {
-  long long start;  // the segment's first tile
+  int start;  // the segment's first tile
   int row, item, tiles, used;
 };
 
@@ -621,7 +642,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   constexpr unsigned long long kAll = ~0ull >> (64 - kTok);
 
   extern __shared__ unsigned char smem_any[];
-  __shared__ unsigned s_scan[kWarps], s_before[kThreads];
+  __shared__ int s_scan[kWarps], s_before[kThreads];
   __shared__ Held s_held[2 * kWarps];
   __shared__ int s_last[2];
   // the swizzle's exclusive-or works on addresses whose rows begin on 128 bytes
@@ -647,7 +668,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
 
   // Where each warp starts: thread i sums the tiles of rows [i n, (i + 1) n).
   const int n = (a.rows + kThreads - 1) / kThreads;
-  unsigned mine = 0;
+  int mine = 0;
   {
     bool bad = false;
     for (int r = tid * n; r < min(a.rows, (tid + 1) * n); ++r) {
@@ -657,25 +678,24 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     }
     if (bad && blockIdx.x == 0) record_device_error(kDevPageRange);
   }
-  unsigned sum = mine;
+  int sum = mine;
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
-    const unsigned x = __shfl_up_sync(0xffffffffu, sum, off);
+    const int x = __shfl_up_sync(0xffffffffu, sum, off);
     if (lane >= off) sum += x;
   }
   if (lane == 31) s_scan[warp] = sum;
   __syncthreads();
-  unsigned before = sum - mine, all = 0;
+  int before = sum - mine, all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_scan[w];
     all += s_scan[w];
   }
   s_before[tid] = before;
-  const long long total = static_cast<long long>(all) * items;
+  const int total = all * items;
   // CTAs in use: no more than give each of their warps a tile, so that short rows are joined within a CTA
-  const long long wanted = (total + kWarps - 1) / kWarps;
-  const int ctas = wanted < gridDim.x ? static_cast<int>(wanted) : gridDim.x;
+  const int ctas = min(static_cast<int>(gridDim.x), (total + kWarps - 1) / kWarps);
   const int cta = blockIdx.x;
   const auto clear_empty_rows = [&]() {
     for (int r = cta; r < a.rows; r += gridDim.x)
@@ -688,9 +708,9 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     return;
   }
   const Shares shares(0, total, ctas);
-  const long long cta_begin = shares.begin(cta), cta_end = shares.begin(cta + 1);
+  const int cta_begin = shares.begin(cta), cta_end = shares.begin(cta + 1);
   const Shares warp_shares(cta_begin, cta_end, kWarps);
-  const long long begin = warp_shares.begin(warp), end = warp_shares.begin(warp + 1);
+  const int begin = warp_shares.begin(warp), end = warp_shares.begin(warp + 1);
   const auto heads_of = [&](int item) { return min(kGroup, a.group - item % a.chunks * kGroup); };
   const auto head_of = [&](int item) { return item / a.chunks * a.group + item % a.chunks * kGroup; };
   __syncthreads();
@@ -699,27 +719,26 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     // the segment of the warp's first tile: in the rows of the last thread that has no more tiles than that before it
     Segment load;  // of the tile to be loaded next
     {
-      unsigned at = static_cast<unsigned>(quotient(begin, items));
+      const int row_tile = begin / items;  // were every row one item
       int owner = -1;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) owner += __popc(__ballot_sync(0xffffffffu, s_before[32 * k + lane] <= at));
-      at -= s_before[owner];
-      int r = owner * n;
+      for (int k = 0; k < kWarps; ++k) owner += __popc(__ballot_sync(0xffffffffu, s_before[32 * k + lane] <= row_tile));
+      int before_row = s_before[owner], r = owner * n;
       Row row = row_of(a, r);
-      while (at >= static_cast<unsigned>((row.tokens + kTok - 1) / kTok) && r + 1 < a.rows) {
-        at -= (row.tokens + kTok - 1) / kTok;
+      int tiles = (row.tokens + kTok - 1) / kTok;
+      while (row_tile >= before_row + tiles && r + 1 < a.rows) {
+        before_row += tiles;
         row = row_of(a, ++r);
+        tiles = (row.tokens + kTok - 1) / kTok;
       }
-      const int tiles = max(1, (row.tokens + kTok - 1) / kTok);
-      const long long start = (quotient(begin, items) - at) * items;  // of the row's first item
-      const int item = min(items - 1, static_cast<int>(quotient(begin - start, tiles)));
-      load = Segment{start + static_cast<long long>(item) * tiles, r, item, row.seq, tiles, row.tokens};
+      const int start = before_row * items, item = min(items - 1, (begin - start) / max(1, tiles));
+      load = Segment{start + item * tiles, r, item, row.seq, tiles, row.tokens};
     }
-    long long load_at = begin;
+    int load_at = begin;
     long long place[kPer];  // bytes from the layer's first element to the lane's tokens of that tile; -1: none
     unsigned long long live = 0;
     const auto look_up = [&]() {
-      const int t0 = static_cast<int>(load_at - load.start) * kTok;
+      const int t0 = (load_at - load.start) * kTok;
       const int* table = a.page_table + load.seq * a.table_stride;
       const long long head = load.item / a.chunks * cache.head_stride;
 #pragma unroll
@@ -787,9 +806,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const auto next_slot = [](int s) { return s + 1 == kSlots ? 0 : s + 1; };
 
     Math math;
-    typename Math::Queries raw;
     look_up();
-    math.ask(raw, a.q + load.row * a.q_stride + static_cast<long long>(head_of(load.item)) * dim, heads_of(load.item), dim);
     find_live();
     fill(0, cache.k);
     cp_async_commit();
@@ -800,7 +817,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     advance();
     if (load_at < end) look_up();
     int slot = 0;
-    for (long long at = begin; at < end; ++at) {
+    for (int at = begin; at < end; ++at) {
       // a slot is filled again as soon as all lanes are done with it: two tiles' halves are under way while a third
       // is worked on
       __syncwarp();
@@ -813,10 +830,8 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       cp_async_commit();
       const int heads = heads_of(now.item);
       const long long first = static_cast<long long>(head_of(now.item)) * dim;
-      if (at == begin || at == now.start) {
-        if (at != begin) math.ask(raw, a.q + now.row * a.q_stride + first, heads, dim);
-        math.begin(raw, a.scale, scratch);
-      }
+      // the queries come while the keys do
+      if (at == begin || at == now.start) math.begin(a.q + now.row * a.q_stride + first, heads, dim, a.scale, scratch);
       cp_async_wait<2>();
       __syncwarp();
       math.scores(smem_u32(ring) + slot * kSlotBytes, now_live, scratch);
@@ -832,7 +847,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       cp_async_wait<2>();
       __syncwarp();
       math.outputs(smem_u32(ring) + value_slot * kSlotBytes, scratch);
-      const long long after = now.start + now.tiles;
+      const int after = now.start + now.tiles;
       if (at + 1 == after || at + 1 == end) {
         if (now.start >= begin && after <= end) {
           math.store(a.out + now.row * a.out_stride + first, heads, dim);
@@ -859,7 +874,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   if (lane < 2 * kWarps) held = s_held[lane];
   const unsigned used = __ballot_sync(0xffffffffu, held.used != 0);
   const unsigned below = used & ((1u << lane) - 1);
-  const long long left = __shfl_sync(0xffffffffu, held.start, below ? 31 - __clz(below) : lane);
+  const int left = __shfl_sync(0xffffffffu, held.start, below ? 31 - __clz(below) : lane);
   const unsigned firsts = __ballot_sync(0xffffffffu, held.used != 0 && (below == 0 || left != held.start));
   const int groups = __popc(firsts);
   const auto members_of = [&](int from) {  // of the group that begins at piece `from`
@@ -997,12 +1012,12 @@ int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& c
   auto kernel = paged_attention_kernel<Math, T, kDim>;
   e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (e != cudaSuccess) return check_cuda(e);
-  const long long most = static_cast<long long>(op.rows) * cache.kv_heads * a.chunks;
-  const long long tiles = (a.room + Math::kTok - 1) / Math::kTok;
-  if (op.rows * tiles >> 32) return set_status(MLI_ERR_UNSUPPORTED);  // tiles are counted in 32 bits
-  // no more CTAs than tiles can be
-  int grid = dev.sm_count < kMaxCtas ? dev.sm_count : kMaxCtas;
-  if (most < grid && most * tiles < grid) grid = static_cast<int>(most * tiles);
+  // tiles, were every row as long as its page table; they are counted in ints
+  const double most = static_cast<double>(op.rows) * cache.kv_heads * a.chunks *
+                      static_cast<double>((a.room + Math::kTok - 1) / Math::kTok);
+  if (most > 2e9) return set_status(MLI_ERR_UNSUPPORTED);
+  const int sms = dev.sm_count < kMaxCtas ? dev.sm_count : kMaxCtas;
+  const int grid = most < sms ? static_cast<int>(most) : sms;
   return check_cuda(
       launch(kernel, dim3(grid), dim3(kWarps * 32), kSmem, stream, true, a, cache_layer<T>(cache, layer)));
 }
