@@ -469,12 +469,13 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
  * has outputs that are not).  Slots behind a row's length are not read.  A row of length <= 0 is
  * zero.  A length beyond the page table is cut to it, keys of a page outside
  * the cache are left out, and a row whose seq lies outside the table is zero;
- * each records device error 6.  rows * kv_heads times the page table's tokens in a
- * row stay below 3e10 (MLI_ERR_UNSUPPORTED).
+ * each records device error 6.  rows * kv_heads * (tokens
+ * that a page-table row can name / 8) stay below 2e9 (MLI_ERR_UNSUPPORTED at worst).
  * `workspace`: mli_paged_attention_workspace_bytes bytes of device memory, 16-byte aligned,
  * zeroed once before its first use; every call leaves it ready for the next,
  * of any sizes that need no more bytes.  Calls that share a workspace must not overlap on the
- * GPU.  Results do not change from run to run.  q and out 16-byte aligned, strides multiples of 4 floats. */
+ * GPU.  Results do not change from run to run.  q and out 16-byte aligned, strides
+ * multiples of 4 floats; out may be q (same stride). */
 typedef struct mli_attention_op {
   int rows, heads;
   float scale;           /* > 0 */

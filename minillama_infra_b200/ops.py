@@ -373,6 +373,8 @@ def _head_rows(t, name, rows, heads, dim, device):
         raise ValueError(f"{name}: expected [{rows}, {heads}, {dim}], got {list(t.shape)}")
     if t.dtype is not _Torch.f32 or t.get_device() != device:
         raise ValueError(f"{name}: expected an fp32 tensor on the cache's device")
+    if t.is_contiguous():
+        return t.data_ptr(), heads * dim
     row, head, one = t.stride()
     if (one != 1 and dim > 1) or (head != dim and heads > 1):
         raise ValueError(f"{name}: expected contiguous heads within a row")
@@ -465,7 +467,7 @@ def paged_attention(out, q, cache: KvCache, layer: int, page_table, lengths, sca
     """Attention of one new token a row over layer `layer` of a paged cache
     (mli_paged_attention; the reference's fused_attention_kernel, :291-365).
 
-    q, out [rows, heads, dim] fp32; lengths int32 [rows], tokens of each row's
+    q, out [rows, heads, dim] fp32 (out may be q); lengths int32 [rows], tokens of each row's
     cache, the new one included (<= 0: the row is zero); seq int32 [rows], the
     row's row of page_table (None: its own number).  workspace:
     paged_attention_workspace; calls that share one must not overlap.

@@ -618,6 +618,73 @@ def test_back_to_back_calls_see_each_other():
             check_row(outs[i][r], qs[i][r], k, v, 0.125)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_attention_in_place(dtype):
+    """out is q, over rows that one CTA, several, and none work on."""
+    g = gen(19)
+    lengths = [9000, 1, 0, 40, 2000]
+    c, table, kv = filled(g, lengths, 2, 16, 64, dtype)
+    q = normal(g, 5, 8, 64)
+    want = attend(c, table, q, i32(lengths), 0.125)
+    ws = ops.paged_attention_workspace(c, 5, 8)
+    ops.paged_attention(q, q, c, 0, table, i32(lengths), 0.125, ws)
+    assert torch.equal(q.view(torch.int32), want.view(torch.int32))
+
+
+def test_one_workspace_for_calls_of_all_sizes():
+    """Calls of other head sizes, row counts and types between two of the same: the same bits."""
+    g = gen(20)
+    cases = []
+    for lengths, heads, group, dim, dtype in (([5000], 8, 8, 256, F32), ([3] * 700, 2, 4, 64, BF16),
+                                              ([4000, 17], 4, 5, 128, F16), ([20000], 1, 16, 64, BF16)):
+        c, table, kv = filled(g, lengths, heads, 16, dim, dtype)
+        cases.append((c, table, kv, normal(g, len(lengths), heads * group, dim), i32(lengths), lengths))
+    ws = max((ops.paged_attention_workspace(c, q.shape[0], q.shape[1]) for c, _, _, q, _, _ in cases), key=len)
+    seen = {}
+    for turn in (0, 1, 2, 3, 1, 0, 3, 2):
+        c, table, kv, q, lengths, plain = cases[turn]
+        got = attend(c, table, q, lengths, q.shape[2] ** -0.5, ws=ws)
+        if turn in seen:
+            assert torch.equal(got.view(torch.int32), seen[turn].view(torch.int32))
+        else:
+            seen[turn] = got
+            for r in (0, len(plain) - 1):
+                check_row(got[r], q[r], *kv[r], q.shape[2] ** -0.5)
+
+
+def test_many_short_rows():
+    """More rows than threads, some without tokens, all of one sequence."""
+    g = gen(21)
+    c, table, kv = filled(g, [70], 2, 16, 64, BF16)
+    rows = 3001
+    lengths = [(7 * r) % 71 for r in range(rows)]
+    q = normal(g, rows, 4, 64)
+    got = attend(c, table, q, i32(lengths), 0.125, seq=torch.zeros(rows, dtype=torch.int32, device="cuda"))
+    for r in list(range(0, rows, 97)) + [rows - 1]:
+        check_row(got[r], q[r], kv[0][0][:lengths[r]], kv[0][1][:lengths[r]], 0.125, f"row {r}")
+    empty = torch.tensor([n == 0 for n in lengths], device="cuda")
+    assert (got[empty] == 0).all() and ops.device_error() == 0
+
+
+def test_two_streams_at_once():
+    """Two calls under way at once, each with its own workspace, on streams that are not the current one."""
+    g = gen(22)
+    c, table, kv = filled(g, [3000, 2500, 100], 2, 16, 64, BF16)
+    qs = [normal(g, 3, 8, 64) for _ in range(2)]
+    lengths = i32([3000, 2500, 100])
+    want = [attend(c, table, q, lengths, 0.125) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ws = [ops.paged_attention_workspace(c, 3, 8) for _ in range(2)]
+    outs = [torch.empty_like(q) for q in qs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i in range(2):
+            ops.paged_attention(outs[i], qs[i], c, 0, table, lengths, 0.125, ws[i], stream=streams[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i].view(torch.int32), want[i].view(torch.int32))
+
+
 def test_refusals_name_the_call():
     g = gen(18)
     c, table, _ = filled(g, [20], 2, 16, 64, BF16)
