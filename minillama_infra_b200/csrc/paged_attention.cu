@@ -914,14 +914,27 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     if (h >= heads_of(g.item)) continue;
     float sum_l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (unsigned rest = members; rest;) {  // four at a time
+      float w[4], l[4];
+      float4 v[4];
+      const int count = __popc(rest);
 #pragma unroll
-    for (int j = 0; j < 2 * kWarps; ++j)
-      if ((members >> j) & 1) {
-        const float w = piece_at(j)->weight[h];
-        const float4 v = *reinterpret_cast<const float4*>(&piece_at(j)->o[h][e]);
-        sum_l = fmaf(w, piece_at(j)->l[h], sum_l);
-        y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
+      for (int u = 0; u < 4; ++u) {
+        const Part& x = *piece_at(rest ? __ffs(rest) - 1 : from);
+        w[u] = x.weight[h];
+        l[u] = x.l[h];
+        v[u] = *reinterpret_cast<const float4*>(&x.o[h][e]);
+        rest &= rest - 1;
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (u >= count) continue;
+        sum_l = fmaf(w[u], l[u], sum_l);
+        y = make_float4(fmaf(w[u], v[u].x, y.x), fmaf(w[u], v[u].y, y.y), fmaf(w[u], v[u].z, y.z),
+                        fmaf(w[u], v[u].w, y.w));
+      }
+    }
     if (g.start >= cta_begin && g.start + g.tiles <= cta_end) {
       const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
       if (e < dim)
