@@ -4,8 +4,8 @@ The compute lives in hand-written CUDA behind a C ABI (include/mli_gemv.h,
 lib/libmli_gemv.so) plus a drop-in shim with the reference's own launcher
 signatures (lib/libmli_dropin.so).  This package holds the build recipe, the
 ctypes binding, torch-tensor wrappers named like the reference launchers
-(``ops``), seeded synthetic workloads (``synth``) and the row-sharded
-multi-GPU classifier (``shard``).
+(``ops``), the pages of a key-value cache (``kv_cache``), seeded synthetic
+workloads (``synth``) and the row-sharded multi-GPU classifier (``shard``).
 """
 import os
 import subprocess

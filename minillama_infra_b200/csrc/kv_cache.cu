@@ -38,6 +38,9 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
 // kQuads times four values each; a warp's heads go in batches whose reads are all under way while the CTA computes
 // its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
 // values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
+// 8192 tokens of 24 / 8 heads of 128 into a bf16 cache: 52 us, 5.78 TB/s of 302 MB (copies run at 6.48); 64 tokens with
+// norms 4.1 us, one token 2.9 us.  1999 tokens of 35 / 5 heads of 80 with norms, 20 of 32 lanes in use: 20 us,
+// 2.7 TB/s, bound by its instructions.
 template <typename T, int kLanes, int kQuads, Partner kPartner>
 __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
   __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
@@ -215,7 +218,8 @@ struct CopyArgs {
   int pages, inner, row, total;                                     // pieces of a row, of a page
 };
 
-// One CTA per (pair, layer, keys or values); bound by HBM, reads and writes alike.
+// One CTA per (pair, layer, keys or values); bound by HBM, reads and writes alike: 256 pages of 16 tokens, 28 layers of
+// 8 heads of 128 in bf16 (470 MB), 144 us, 6.53 TB/s read and written; 4 pages of 16 layers of 8 heads of 64, 2.4 us.
 template <bool kWhole>  // a page is one row
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs a, const int* src, const int* dst) {
   griddep_wait();
