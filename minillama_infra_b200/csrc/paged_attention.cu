@@ -731,8 +731,13 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   const int cta_begin = shares.begin(cta), cta_end = shares.begin(cta + 1);
   const Shares warp_shares(cta_begin, cta_end, kWarps);
   const int begin = warp_shares.begin(warp), end = warp_shares.begin(warp + 1);
-  const auto heads_of = [&](int item) { return min(kGroup, a.group - item % a.chunks * kGroup); };
-  const auto head_of = [&](int item) { return item / a.chunks * a.group + item % a.chunks * kGroup; };
+  // an item's key-value head, its first query head, and how many it has
+  const auto kv_head_of = [&](int item) { return a.chunks == 1 ? item : item / a.chunks; };
+  const auto head_of = [&](int item) {
+    const int kv = kv_head_of(item);
+    return kv * a.group + (item - kv * a.chunks) * kGroup;
+  };
+  const auto heads_of = [&](int item) { return min(kGroup, a.group - (item - kv_head_of(item) * a.chunks) * kGroup); };
   __syncthreads();
 
   if (begin < end) {
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     const auto look_up = [&]() {
       const int t0 = (load_at - load.start) * kTok;
       const int* table = a.page_table + load.seq * a.table_stride;
-      const long long head = load.item / a.chunks * cache.head_stride;
+      const long long head = kv_head_of(load.item) * cache.head_stride;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int t = t0 + lane + 32 * i;
@@ -848,10 +853,10 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
         fill(free_slot, cache.k);
       }
       cp_async_commit();
-      const int heads = heads_of(now.item);
-      const long long first = static_cast<long long>(head_of(now.item)) * dim;
       // the queries come while the keys do
-      if (at == begin || at == now.start) math.begin(a.q + now.row * a.q_stride + first, heads, dim, a.scale, scratch);
+      if (at == begin || at == now.start)
+        math.begin(a.q + now.row * a.q_stride + static_cast<long long>(head_of(now.item)) * dim, heads_of(now.item), dim,
+                   a.scale, scratch);
       cp_async_wait<2>();
       __syncwarp();
       math.scores(smem_u32(ring) + slot * kSlotBytes, now_live, scratch);
@@ -870,7 +875,8 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       const int after = now.start + now.tiles;
       if (at + 1 == after || at + 1 == end) {
         if (now.start >= begin && after <= end) {
-          math.store(a.out + now.row * a.out_stride + first, heads, dim);
+          math.store(a.out + now.row * a.out_stride + static_cast<long long>(head_of(now.item)) * dim,
+                     heads_of(now.item), dim);
         } else {
           const int h = 2 * warp + (at + 1 == end);
           __syncwarp();  // every lane has read its last values
