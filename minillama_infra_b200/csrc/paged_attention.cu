@@ -28,13 +28,13 @@
 // Bound by HBM: 4 products a 16-bit value read with 4 query heads a key-value
 // head.  Measured on one B200 whose copies run at 6.48 TB/s, calls captured one after
 // another, data not in L2:
-//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         96 us   5.60 TB/s
-//   64 rows of 0..8192 tokens, same heads                     176 us   6.09 TB/s
-//   64 rows of 4096, 64 / 8 heads of 128, bf16                174 us   6.19 TB/s
-//   32 rows of 4096, 32 / 4 heads of 256, bf16                121 us   4.46 TB/s
-//   64 rows of 2048, 32 / 8 heads of 128, fp32                167 us   6.43 TB/s
-//   64 rows of 2048, 64 / 8 heads of 128, fp32                249 us   4.32 TB/s
-//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               20 us   3.46 TB/s
+//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         95 us   5.63 TB/s
+//   64 rows of 0..8192 tokens, same heads                     174 us   6.16 TB/s
+//   64 rows of 4096, 64 / 8 heads of 128, bf16                178 us   6.06 TB/s
+//   32 rows of 4096, 32 / 4 heads of 256, bf16                115 us   4.69 TB/s
+//   64 rows of 2048, 32 / 8 heads of 128, fp32                172 us   6.24 TB/s
+//   64 rows of 2048, 64 / 8 heads of 128, fp32                237 us   4.54 TB/s
+//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.57 TB/s
 //   1 row of 53, 32 / 8 heads of 64, fp32                       7 us
 // Equal shares do not end at once (63 to 89 us for the first line: SMs get unequal bandwidth), and
 // a call's first bytes are asked for after 2.5 us (lengths, the search of each warp's
@@ -218,8 +218,10 @@ struct TensorMath {
   static constexpr int kTok = kSlotBytes / (kDim * 2);  // 64, 32 or 16 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kSteps = kUsed / 16;
-  // the third parts of 8 heads of 256 queries would not fit in registers beside the rest: they are in shared memory
-  static constexpr bool kThirdShared = kDim == 256 && !kFew;
+  // The third parts of 8 heads' queries of 128 dims and more do not fit in registers beside the rest: they are in shared
+  // memory, which costs a warp (64 rows of 4096, 64 / 8 heads of 128: 178 us, spilling them 180; 32 rows, 32 / 4 heads
+  // of 256: 121 and 215).
+  static constexpr bool kThirdShared = kUsed >= 128 && !kFew;
   static constexpr int kScratch = kThirdShared ? kSteps * 64 : 0;
   static constexpr int kReadBytes = kUsed * 2;  // of a token
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;

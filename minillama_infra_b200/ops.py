@@ -402,9 +402,10 @@ def _table(t, device):
 
 
 def _rows_and_heads(q):
-    if len(q.shape) != 3:
-        raise ValueError(f"q: expected [rows, heads, head_dim], got {list(q.shape)}")
-    return q.shape[:2]
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"q: expected [rows, heads, head_dim], got {list(shape)}")
+    return shape[0], shape[1]
 
 
 def rope_turns(rot_dim: int, theta: float = 500000.0, scaling: str = "none", factor: float = 1.0,
