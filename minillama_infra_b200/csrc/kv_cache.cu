@@ -198,9 +198,10 @@ int launch_append(const mli_rope_op& op, const mli_kv_cache& cache, int layer, c
   const auto kernel = dim <= 64    ? append_kernel<T, 16, 1>(partner)
                       : dim <= 128 ? append_kernel<T, 32, 1>(partner)
                                    : append_kernel<T, 32, 2>(partner);
-  // few tokens: their heads over as many CTAs as give each warp one turn, or as fill the SMs four times
-  const int at_once = kAppendWarps * (dim <= 64 ? 2 : 1), heads = op.heads + 2 * cache.kv_heads;
-  const int most = (heads + at_once - 1) / at_once, fill = 4 * dev.sm_count / op.m;
+  // Few tokens: their heads over as many CTAs as put eight on an SM, of four turns a warp at least (500 tokens of 32 / 8
+  // heads of 128 with norms 7.9 us, with four on an SM 11.0; 64 tokens 4.0 us, with one turn a warp 5.9).
+  const int turn = kAppendWarps * (dim <= 64 ? 2 : 1), heads = op.heads + 2 * cache.kv_heads;
+  const int most = (heads + 4 * turn - 1) / (4 * turn), fill = 8 * dev.sm_count / op.m;
   const int share = fill < 1 ? 1 : fill < most ? fill : most;
   const dim3 grid(static_cast<unsigned>(op.m), static_cast<unsigned>(share));
   return check_cuda(launch(kernel, grid, dim3(kAppendThreads), 0, stream, true, op, cache_layer<T>(cache, layer)));
