@@ -39,7 +39,7 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
 // its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
 // values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
 // 8192 tokens of 24 / 8 heads of 128 into a bf16 cache: 52 us, 5.78 TB/s of 302 MB (copies run at 6.48); 64 tokens with
-// norms 4.1 us, one token 2.9 us.  1999 tokens of 35 / 5 heads of 80 with norms, 20 of 32 lanes in use: 20 us,
+// norms 3.9 us, one token 2.8 us.  1999 tokens of 35 / 5 heads of 80 with norms, 20 of 32 lanes in use: 20 us,
 // 2.7 TB/s, bound by its instructions.
 template <typename T, int kLanes, int kQuads, Partner kPartner>
 __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
