@@ -29,12 +29,12 @@
 // head.  Measured on one B200 whose copies run at 6.48 TB/s, calls captured one after
 // another, data not in L2:
 //   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         95 us   5.63 TB/s
-//   64 rows of 0..8192 tokens, same heads                     174 us   6.16 TB/s
-//   64 rows of 4096, 64 / 8 heads of 128, bf16                178 us   6.06 TB/s
+//   64 rows of 0..8192 tokens, same heads                     174 us   6.13 TB/s
+//   64 rows of 4096, 64 / 8 heads of 128, bf16                176 us   6.12 TB/s
 //   32 rows of 4096, 32 / 4 heads of 256, bf16                115 us   4.69 TB/s
-//   64 rows of 2048, 32 / 8 heads of 128, fp32                172 us   6.24 TB/s
+//   64 rows of 2048, 32 / 8 heads of 128, fp32                169 us   6.36 TB/s
 //   64 rows of 2048, 64 / 8 heads of 128, fp32                237 us   4.54 TB/s
-//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.57 TB/s
+//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.64 TB/s
 //   1 row of 53, 32 / 8 heads of 64, fp32                       7 us
 // Equal shares do not end at once (63 to 89 us for the first line: SMs get unequal bandwidth), and
 // a call's first bytes are asked for after 2.5 us (lengths, the search of each warp's
@@ -127,7 +127,7 @@ template <int kDim, int kHeads>
 struct Piece {
   float o[kHeads][kDim];
   float m[kHeads], l[kHeads], c[kHeads];
-  float weight[kHeads];  // beside the other pieces of its CTA
+  float weight[kHeads], top[kHeads];  // beside the other pieces of its CTA, and their maximum
 };
 // What a piece of maximum m counts beside one of maximum top (no piece: 1, and its sums are zero).
 __device__ __forceinline__ float piece_weight(float m, float top, float c) {
@@ -646,7 +646,8 @@ struct Held {
 };
 
 // Bytes of a warp, and how many of them an SM's 227 KB hold beside the static arrays and 128 bytes for alignment.
-constexpr int kSmemRoom = 232448 - 1792 - 128;
+constexpr int kStaticBytes = 1408;
+constexpr int kSmemRoom = 232448 - kStaticBytes - 128;
 template <typename Math>
 constexpr int kWarpBytes = kSlots * kSlotBytes + sizeof(typename Math::Part) + Math::kScratch * 4;
 template <typename Math>
@@ -667,6 +668,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
   __shared__ int s_scan[kWarps], s_before[kThreads];
   __shared__ Held s_held[2 * kWarps];
   __shared__ int s_last[2];
+  static_assert(sizeof(s_scan) + sizeof(s_before) + sizeof(s_held) + sizeof(s_last) <= kStaticBytes, "static arrays");
   // the swizzle's exclusive-or works on addresses whose rows begin on 128 bytes
   unsigned char* smem = smem_any + (-smem_u32(smem_any) & 127u);
   // rings, then a piece of each warp, then its scratch.  A warp's second piece takes its ring, which is empty by then.
@@ -918,6 +920,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
 #pragma unroll
     for (int k = 0; k < 2 * kWarps; ++k) top = fmaxf(top, (members >> k) & 1 ? piece_at(k)->m[h] : -INFINITY);
     piece_at(j)->weight[h] = piece_weight(piece_at(j)->m[h], top, piece_at(j)->c[h]);
+    piece_at(j)->top[h] = top;
   }
   __syncthreads();
   const auto group_lane = [&](int g) {
@@ -972,9 +975,7 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
       Part* to = parts + 2 * cta + (g.start > cta_begin ? 1 : 0);
       *reinterpret_cast<float4*>(&to->o[h][e]) = y;
       if (e == 0) {
-        float top = -INFINITY;
-        for (unsigned b = members; b; b &= b - 1) top = fmaxf(top, piece_at(__ffs(b) - 1)->m[h]);
-        to->m[h] = top;
+        to->m[h] = piece_at(from)->top[h];
         to->l[h] = sum_l;
         to->c[h] = piece_at(from)->c[h];
       }
@@ -1082,7 +1083,7 @@ int launch_attention(const Args& a, const mli_attention_op& op, const mli_kv_cac
   const int dim = cache.head_dim;
   if (dim <= 64) return launch_dim<T, 64, 64>(a, op, cache, layer, s);
   // the tensor cores' share of a call goes by the dims they multiply: 80 and 96 have kernels of their own
-  // (64 rows of 2048, 64 / 8 heads: 69 and 77 us, with the kernel for 128 90 and 91 us; with 32 / 8 heads, bound by
+  // (64 rows of 2048, 64 / 8 heads: 66 and 74 us, with the kernel for 128 90 and 91 us; with 32 / 8 heads, bound by
   // HBM, 64 us against 68 for 80, 137 against 134 for 96)
   if constexpr (sizeof(T) == 2) {
     if (dim <= 80) return launch_dim<T, 128, 80>(a, op, cache, layer, s);
