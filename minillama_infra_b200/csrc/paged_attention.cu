@@ -1046,6 +1046,10 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
 
 template <typename Math, typename T, int kDim>
 int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t stream) {
+  // tiles, were every row as long as its page table; they are counted in ints
+  const double most = static_cast<double>(op.rows) * cache.kv_heads * a.chunks *
+                      static_cast<double>((a.room + Math::kTok - 1) / Math::kTok);
+  if (most > 2e9) return set_status(MLI_ERR_UNSUPPORTED);
   cudaError_t e = cudaSuccess;
   const DeviceInfo& dev = current_device(&e);
   if (e != cudaSuccess) return check_cuda(e);
@@ -1054,10 +1058,6 @@ int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& c
   auto kernel = paged_attention_kernel<Math, T, kDim>;
   e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (e != cudaSuccess) return check_cuda(e);
-  // tiles, were every row as long as its page table; they are counted in ints
-  const double most = static_cast<double>(op.rows) * cache.kv_heads * a.chunks *
-                      static_cast<double>((a.room + Math::kTok - 1) / Math::kTok);
-  if (most > 2e9) return set_status(MLI_ERR_UNSUPPORTED);
   const int sms = dev.sm_count < kMaxCtas ? dev.sm_count : kMaxCtas;
   const int grid = most < sms ? static_cast<int>(most) : sms;
   return check_cuda(

@@ -94,6 +94,16 @@ def test_layers_null_structs_and_counts_are_refused():
     assert l.mli_kv_copy_pages(c, A, A, 0, None) == INVALID
 
 
+def test_sizes_beyond_the_kernels_counters_are_refused():
+    """More tiles than an int counts; pages of more 16-byte pieces than one does; more layers than a grid has."""
+    l, c = _lib.lib(), cache()
+    wide = dict(table_cols=1 << 27, table_stride=1 << 27)  # of 64 tokens a tile: 2^25 tiles a row and head
+    assert l.mli_paged_attention(attention(rows=1 << 10, **wide), c, 0, None) == UNSUPPORTED
+    assert l.mli_paged_attention(attention(rows=1 << 20, table_cols=1 << 13, table_stride=1 << 13), c, 0, None) == UNSUPPORTED
+    assert l.mli_kv_copy_pages(cache(page_size=1 << 23), A, A, 1, None) == UNSUPPORTED
+    assert l.mli_kv_copy_pages(cache(layers=65536), A, A, 1, None) == UNSUPPORTED
+
+
 def test_workspace_bytes():
     size = _lib.lib().mli_paged_attention_workspace_bytes
     assert size(1, 8, 8, 64) > 0
