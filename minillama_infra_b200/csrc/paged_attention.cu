@@ -420,56 +420,76 @@ struct TensorMath {
   }
 };
 
-// ---- the products in fp32, fp32 caches ----------------------------------------
-//
-// A lane takes a part of the dims of two tokens for the scores and four dims of a token
-// (or eight) for the outputs; q and p come from shared memory as broadcasts.
 __device__ __forceinline__ const float4* shared_float4(unsigned addr) {
   return reinterpret_cast<const float4*>(__cvta_shared_to_generic(addr));
 }
 
+// ---- the products in fp32, fp32 caches ----------------------------------------
+//
+// A lane takes a part of the dims of two tokens for the scores; the lanes that share a token then share out its heads,
+// each adding up and weighing its own.  For the outputs a lane takes four dims of a token (or eight) of all heads; q, p and
+// the factor of the earlier outputs come from shared memory as broadcasts, p of 8 heads twice over, as the packed
+// products take it.
 template <int kDim, bool kFew>
 struct FloatMath {
   static constexpr int kTok = kSlotBytes / (kDim * 4);  // 32, 16 or 8 tokens a tile
   static constexpr int kHeads = kFew ? 4 : 8;
-  static constexpr int kScratch = kHeads * (kDim + kTok);  // floats: q, then the tile's p
+  static constexpr int kCopies = kFew ? 1 : 2;  // of p
+  static constexpr int kScratch = kHeads * (kDim + kTok * kCopies + 1);  // floats: q, the tile's p, a number a head
   static constexpr int kReadBytes = kDim * 4;  // of a token
-  static constexpr int kLanes = kTok / 2;    // side by side in the scores, two tokens each
-  static constexpr int kParts = 32 / kLanes;  // lanes that share a token's dims
-  static constexpr int kChunks = kDim / 4;   // 16-byte pieces of a token
+  static constexpr int kLanes = kTok / 2;      // side by side in the scores, two tokens each
+  static constexpr int kParts = 32 / kLanes;   // lanes that share a token's dims, then its heads
+  static constexpr int kMine = kHeads > kParts ? kHeads / kParts : 1;  // heads of a lane
+  static constexpr int kChunks = kDim / 4;     // 16-byte pieces of a token
   static constexpr int kRows = kChunks < 32 ? 32 / kChunks : 1;  // tokens side by side in the outputs' sum
   static constexpr int kOwn = kChunks < 32 ? 1 : kChunks / 32;   // pieces of a token a lane sums
 
   using Part = Piece<kDim, kHeads>;
 
   float2 o[kHeads][kOwn][2];
-  float m[kHeads], l[kHeads], keep[kHeads], c;
+  float m[kMine], l[kMine], c;
+  float* per_head;  // kHeads numbers in shared memory
+  int base_head;    // this lane's first head
+  bool owner;       // of its heads among lanes with the same tokens and heads
 
   __device__ __forceinline__ void begin(const float* qp, int heads, int dim, float scale, float* scratch) {
+    const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < kHeads * kChunks / 32; ++k) {
-      const int i = (threadIdx.x & 31) + 32 * k, h = i / kChunks, e = 4 * (i % kChunks);
+      const int i = lane + 32 * k, h = i / kChunks, e = 4 * (i % kChunks);
       reinterpret_cast<float4*>(scratch)[i] = h < heads && e < dim
                                                   ? *reinterpret_cast<const float4*>(qp + h * dim + e)
                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
     c = scale;
+    per_head = scratch + kHeads * (kDim + kTok * kCopies);
+    base_head = 0;
+    owner = true;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int off = 16, half = kHeads / 2; off >= kLanes; off /= 2, half /= 2) {
+      if (half > 0)
+        base_head += lane & off ? half : 0;
+      else
+        owner = owner && !(lane & off);
+    }
+#pragma unroll
+    for (int h = 0; h < kMine; ++h) {
       m[h] = -INFINITY;
       l[h] = 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) o[h][i][0] = o[h][i][1] = make_float2(0.f, 0.f);
-    }
   }
 
   __device__ __forceinline__ void scores(unsigned slot, unsigned long long live, float* scratch) {
     const int lane = threadIdx.x & 31;
     const float4* keys = shared_float4(slot);
     const float4* qs = reinterpret_cast<const float4*>(scratch);
-    float4* ps = reinterpret_cast<float4*>(scratch + kHeads * kDim);  // [kTok][kHeads]
+    float* ps = scratch + kHeads * kDim;  // [kTok][kHeads][kCopies]
     const int t = lane % kLanes, part = lane / kLanes;
     float2 acc[2][kHeads][2];
 #pragma unroll
@@ -491,74 +511,113 @@ struct FloatMath {
         acc[1][h][1] = fma2(make_float2(x1.z, x1.w), make_float2(y.z, y.w), acc[1][h][1]);
       }
     }
-    float p[2][kHeads];
+    float s[2][kHeads];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        const float2 x = add2(acc[r][h][0], acc[r][h][1]);
+        s[r][h] = x.x + x.y;
+      }
+    // each exchange adds another lane's part to half of the heads and gives away the other half
+#pragma unroll
+    for (int off = 16, half = kHeads / 2; off >= kLanes; off /= 2, half /= 2) {
+      const bool upper = lane & off;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float s = (acc[r][h][0].x + acc[r][h][0].y) + (acc[r][h][1].x + acc[r][h][1].y);
+        if (half > 0) {
 #pragma unroll
-        for (int off = kLanes; off < 32; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
-        p[r][h] = (live >> (t + r * kLanes)) & 1 ? s : -INFINITY;
+          for (int h = 0; h < half; ++h) {
+            const float kept = upper ? s[r][h + half] : s[r][h], sent = upper ? s[r][h] : s[r][h + half];
+            s[r][h] = kept + __shfl_xor_sync(0xffffffffu, sent, off);
+          }
+        } else {
+          s[r][0] += __shfl_xor_sync(0xffffffffu, s[r][0], off);
+        }
       }
-      float top = fmaxf(p[0][h], p[1][h]);
+    }
+#pragma unroll
+    for (int h = 0; h < kMine; ++h) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) s[r][h] = (live >> (t + r * kLanes)) & 1 ? s[r][h] : -INFINITY;
+      float top = fmaxf(s[0][h], s[1][h]);
 #pragma unroll
       for (int off = kLanes / 2; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       top = fmaxf(top, m[h]);
       const float base = top == -INFINITY ? 0.f : top;
-      keep[h] = exp2_approx((m[h] - base) * c);
+      const float keep = exp2_approx((m[h] - base) * c);
       m[h] = top;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) p[r][h] = exp2_approx((p[r][h] - base) * c);
-      l[h] = fmaf(l[h], keep[h], part == 0 ? p[0][h] + p[1][h] : 0.f);
+      for (int r = 0; r < 2; ++r) s[r][h] = exp2_approx((s[r][h] - base) * c);
+      l[h] = fmaf(l[h], keep, s[0][h] + s[1][h]);
+      if (owner) {
+        if (t == 0) per_head[base_head + h] = keep;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float* to = ps + ((t + r * kLanes) * kHeads + base_head + h) * kCopies;
+          if constexpr (kCopies == 2)
+            *reinterpret_cast<float2*>(to) = make_float2(s[r][h], s[r][h]);
+          else
+            *to = s[r][h];
+        }
+      }
     }
-    if (part == 0)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int h4 = 0; h4 < kHeads / 4; ++h4)
-          ps[(t + r * kLanes) * (kHeads / 4) + h4] =
-              make_float4(p[r][4 * h4], p[r][4 * h4 + 1], p[r][4 * h4 + 2], p[r][4 * h4 + 3]);
     __syncwarp();
   }
 
   __device__ __forceinline__ void outputs(unsigned slot, float* scratch) {
     const int lane = threadIdx.x & 31;
     const float4* values = shared_float4(slot);
-    const float* ps = scratch + kHeads * kDim;
+    const float4* ps = reinterpret_cast<const float4*>(scratch + kHeads * kDim);
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
+    for (int h4 = 0; h4 < kHeads / 4; ++h4) {
+      const float4 k4 = reinterpret_cast<const float4*>(per_head)[h4];
+      const float keep[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i)
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o[h][i][j] = mul2(o[h][i][j], make_float2(keep[h], keep[h]));
+        for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            o[4 * h4 + h][i][j] = mul2(o[4 * h4 + h][i][j], make_float2(keep[h], keep[h]));
+    }
     const int first = kRows > 1 ? lane / kChunks : 0, piece = kRows > 1 ? lane % kChunks : lane;
 #pragma unroll 4
     for (int r = first; r < kTok; r += kRows) {
       float4 x[kOwn];
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) x[i] = values[r * kChunks + ((piece + 32 * i) ^ (r & 7))];
+      constexpr int kReads = kHeads * kCopies / 4, kEach = 4 / kCopies;  // of p, and heads of a read
 #pragma unroll
-      for (int h4 = 0; h4 < kHeads / 4; ++h4) {
-        const float4 p4 = *reinterpret_cast<const float4*>(ps + r * kHeads + 4 * h4);
+      for (int g = 0; g < kReads; ++g) {
+        const float4 p4 = ps[r * kReads + g];
         const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
+        for (int h = 0; h < kEach; ++h)
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) {
-            o[4 * h4 + h][i][0] = fma2(make_float2(p[h], p[h]), make_float2(x[i].x, x[i].y), o[4 * h4 + h][i][0]);
-            o[4 * h4 + h][i][1] = fma2(make_float2(p[h], p[h]), make_float2(x[i].z, x[i].w), o[4 * h4 + h][i][1]);
+            const float2 w = make_float2(p[h * kCopies], p[h * kCopies + kCopies - 1]);
+            float2(&to)[2] = o[g * kEach + h][i];
+            to[0] = fma2(w, make_float2(x[i].x, x[i].y), to[0]);
+            to[1] = fma2(w, make_float2(x[i].z, x[i].w), to[1]);
           }
       }
     }
-    __syncwarp();  // ps is written again by the next tile
+    __syncwarp();  // ps and per_head are written again by the next tile
   }
 
+  // The sums over lanes; after it every lane finds all heads' in per_head.
   __device__ __forceinline__ void finish() {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      l[h] = warp_sum(l[h]);
-      if (kRows > 1) {
+    for (int h = 0; h < kMine; ++h) {
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off /= 2) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+      if (owner && lane % kLanes == 0) per_head[base_head + h] = l[h];
+    }
+    if (kRows > 1) {
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -566,8 +625,8 @@ struct FloatMath {
             o[h][0][j].x += __shfl_xor_sync(0xffffffffu, o[h][0][j].x, off);
             o[h][0][j].y += __shfl_xor_sync(0xffffffffu, o[h][0][j].y, off);
           }
-      }
     }
+    __syncwarp();
   }
   __device__ __forceinline__ void store(float* out, int heads, int dim) {
     finish();
@@ -575,7 +634,7 @@ struct FloatMath {
     if (kRows > 1 && lane >= kChunks) return;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+      const float sum = per_head[h], inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
         const int e = 4 * (lane + 32 * i);
@@ -588,19 +647,20 @@ struct FloatMath {
   __device__ __forceinline__ void store(Part& to) {
     finish();
     const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < kMine; ++h)
+      if (owner && lane % kLanes == 0) {
+        to.m[base_head + h] = m[h];
+        to.l[base_head + h] = l[h];
+        to.c[base_head + h] = c;
+      }
     if (kRows > 1 && lane >= kChunks) return;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
         *reinterpret_cast<float4*>(&to.o[h][4 * (lane + 32 * i)]) =
             make_float4(o[h][i][0].x, o[h][i][0].y, o[h][i][1].x, o[h][i][1].y);
-      if (lane == 0) {
-        to.m[h] = m[h];
-        to.l[h] = l[h];
-        to.c[h] = c;
-      }
-    }
   }
 };
 
