@@ -20,9 +20,9 @@ constexpr int kAppendThreads = kAppendWarps * 32;
 // Where the other value of a rotated pair comes from.
 enum Partner {
   kSameQuad,   // interleaved pairs: the same four values
-  kOtherLane,  // halves of whole quads, one quad a lane
+  kOtherLane,  // halves of whole quads, both within 32 lanes' first quads
   kOtherQuad,  // halves of 32 quads, two quads a lane
-  kReload,     // any other half: read again
+  kExchange,   // any other half: through shared memory
 };
 
 __device__ __forceinline__ void store4(float* p, const float (&y)[4]) {
@@ -43,13 +43,14 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
 // 2.7 TB/s, bound by its instructions.
 template <typename T, int kLanes, int kQuads, Partner kPartner>
 __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
+  constexpr int kAtOnce = 32 / kLanes, kBatch = 4 / kQuads;  // heads of a warp side by side, and after one another
   __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
+  __shared__ float4 s_heads[kPartner == kExchange ? kAppendWarps : 1][kPartner == kExchange ? kBatch : 1][kQuads][32];
   griddep_wait();
   griddep_launch_dependents();
   const int t = blockIdx.x;
   const int pos = op.pos[t];
   if (pos < 0) return;  // padding
-  constexpr int kAtOnce = 32 / kLanes, kBatch = 4 / kQuads;  // heads of a warp side by side, and after one another
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int l = lane % kLanes, sub = lane / kLanes;
   const int dim = c.head_dim, half = op.rot_dim / 2, keys = op.heads, values = op.heads + c.kv_heads;
@@ -145,27 +146,33 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
           y[i][3] *= inv * u.w;
         }
       }
+      if constexpr (kPartner == kExchange) {
+        static_assert(kBatch > 1, "a head's buffer comes round again after the barrier of another");
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+          s_heads[warp][b][i][lane] = make_float4(y[i][0], y[i][1], y[i][2], y[i][3]);
+        __syncwarp();
+      }
       float z[kQuads][4];
 #pragma unroll
       for (int i = 0; i < kQuads; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int e = 4 * (l + 32 * i) + j;
-          float other;
+          float other = 0.f;
           if constexpr (kPartner == kSameQuad) {
             other = y[i][j ^ 1];
           } else if constexpr (kPartner == kOtherLane) {
-            other = __shfl_sync(0xffffffffu, y[i][j], l < half / 4 ? l + half / 4 : l - half / 4, kLanes);
+            if (i == 0) other = __shfl_sync(0xffffffffu, y[i][j], l < half / 4 ? l + half / 4 : l - half / 4, kLanes);
           } else if constexpr (kPartner == kOtherQuad) {
             other = y[i ^ 1][j];
           } else {
-            const int o = e < half ? e + half : e - half;
-            other = h < values && e < op.rot_dim ? source(h)[o] * (inv * (w ? w[o] : 1.f)) : 0.f;
+            const float* head = reinterpret_cast<const float*>(s_heads[warp][b]) + 4 * kLanes * sub;
+            if (e < op.rot_dim) other = head[e < half ? e + half : e - half];
           }
           // behind rot_dim the other value, whatever it is, is not part of the result
           z[i][j] = h >= values ? y[i][j] : fmaf(y[i][j], cs[i][j], (e < op.rot_dim ? other : 0.f) * sn[i][j]);
         }
-      if (kPartner == kReload) __syncwarp();  // q_out may be q, whose values a neighbour reads again
 #pragma unroll
       for (int i = 0; i < kQuads; ++i) {
         if (4 * (l + 32 * i) >= dim) continue;
@@ -180,9 +187,13 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
 
 template <typename T, int kLanes, int kQuads>
 auto append_kernel(Partner partner) {
-  return partner == kSameQuad ? rope_append_kernel<T, kLanes, kQuads, kSameQuad>
-         : partner == kReload ? rope_append_kernel<T, kLanes, kQuads, kReload>
-                              : rope_append_kernel<T, kLanes, kQuads, kQuads == 2 ? kOtherQuad : kOtherLane>;
+  switch (partner) {
+    case kSameQuad: return rope_append_kernel<T, kLanes, kQuads, kSameQuad>;
+    case kOtherLane: return rope_append_kernel<T, kLanes, kQuads, kOtherLane>;
+    case kOtherQuad:
+      if constexpr (kQuads == 2) return rope_append_kernel<T, kLanes, kQuads, kOtherQuad>;
+    default: return rope_append_kernel<T, kLanes, kQuads, kExchange>;
+  }
 }
 
 template <typename T>
@@ -191,10 +202,10 @@ int launch_append(const mli_rope_op& op, const mli_kv_cache& cache, int layer, c
   const DeviceInfo& dev = current_device(&e);
   if (e != cudaSuccess) return check_cuda(e);
   const int half = op.rot_dim / 2, dim = cache.head_dim;
-  const Partner partner = op.interleaved || half == 0                       ? kSameQuad
-                          : dim > 128 ? (half == 128 ? kOtherQuad : kReload)
-                          : half % 4 == 0                                   ? kOtherLane
-                                                                            : kReload;
+  const Partner partner = op.interleaved || half == 0       ? kSameQuad
+                          : half % 4 == 0 && half <= 64     ? kOtherLane
+                          : half == 128                     ? kOtherQuad
+                                                            : kExchange;
   const auto kernel = dim <= 64    ? append_kernel<T, 16, 1>(partner)
                       : dim <= 128 ? append_kernel<T, 32, 1>(partner)
                                    : append_kernel<T, 32, 2>(partner);
