@@ -12,8 +12,8 @@
 namespace mli {
 namespace {
 
-// Two warps: each repeats a token's set-up, so 8192 tokens of 24 / 8 heads of 128 took 57 us with four; with one (52 us)
-// 1999 tokens of 35 / 5 heads of 80 took 31 us instead of 22.
+// Two warps: each repeats a token's set-up, so 8192 tokens of 24 / 8 heads of 128 took 57 us with four and 52 with two;
+// with one (52 us) 1999 tokens of 35 / 5 heads of 80 took 31 us instead of 22.
 constexpr int kAppendWarps = 2;
 constexpr int kAppendThreads = kAppendWarps * 32;
 
@@ -38,10 +38,10 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
 // kQuads times four values each; a warp's heads go in batches whose reads are all under way while the CTA computes
 // its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
 // values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
-// 8192 tokens of 24 / 8 heads of 128 into a bf16 cache: 52 us, 5.78 TB/s of 302 MB (copies run at 6.48); 64 tokens with
-// norms 3.9 us, one token 2.8 us.  1999 tokens of 35 / 5 heads of 80 with norms, 20 of 32 lanes in use: 20 us,
-// 2.7 TB/s, bound by its instructions.
-template <typename T, int kLanes, int kQuads, Partner kPartner>
+// 8192 tokens of 24 / 8 heads of 128 into a bf16 cache: 51 us, 5.90 TB/s of 302 MB (copies run at 6.48); 64 tokens with
+// norms 3.9 us, one token 2.7 us.  With norms the instructions bind: 4096 tokens of 32 / 8 heads of 128 38 us, 4.81 TB/s;
+// 1999 tokens of 35 / 5 heads of 80, 20 of 32 lanes in use, 18 us, 3.0 TB/s.
+template <typename T, int kLanes, int kQuads, Partner kPartner, bool kNorms>
 __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
   constexpr int kAtOnce = 32 / kLanes, kBatch = 4 / kQuads;  // heads of a warp side by side, and after one another
   __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
@@ -108,13 +108,43 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
       cs[i][j] = on ? s_cos[pair] : 1.f;
       sn[i][j] = on ? (second ? s_sin[pair] : -s_sin[pair]) : 0.f;
     }
-  const bool norms = op.q_norm || op.k_norm;
   const float per_dim = 1.f / dim;
   float* const q_to = op.q_out + t * op.q_out_stride + 4 * l;
   T* const k_to = c.k + slot + 4 * l;
   T* const v_to = c.v + slot + 4 * l;
 
   for (; first < total; first += kBatch * step, read(first)) {
+    float inv[kBatch];
+    if constexpr (kNorms) {
+      // the batch's sums of squares together: an exchange adds another lane's to half of the heads and gives away the
+      // other half, until a lane has one head's, whose root it takes for all
+      float ss[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        ss[b] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+          const float4 v = x[b][i];
+          ss[b] += (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w);
+        }
+      }
+#pragma unroll
+      for (int off = kLanes / 2, n = kBatch / 2; off > 0; off /= 2, n /= 2) {
+        if (n > 0) {
+          const bool upper = l & off;
+#pragma unroll
+          for (int b = 0; b < n; ++b) {
+            const float kept = upper ? ss[b + n] : ss[b], sent = upper ? ss[b] : ss[b + n];
+            ss[b] = kept + __shfl_xor_sync(0xffffffffu, sent, off);
+          }
+        } else {
+          ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], off);
+        }
+      }
+      const float root = rsqrtf(ss[0] * per_dim + op.eps);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) inv[b] = __shfl_sync(0xffffffffu, root, b * (kLanes / kBatch), kLanes);
+    }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = first + b * step + sub;
@@ -127,23 +157,15 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
         y[i][3] = x[b][i].w;
       }
       const float* w = h < keys ? op.q_norm : h < values ? op.k_norm : nullptr;
-      float inv = 1.f;
-      if (norms) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i)
-          ss += (y[i][0] * y[i][0] + y[i][1] * y[i][1]) + (y[i][2] * y[i][2] + y[i][3] * y[i][3]);
-#pragma unroll
-        for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        if (w) inv = rsqrtf(ss * per_dim + op.eps);
+      if (kNorms && w) {
 #pragma unroll
         for (int i = 0; i < kQuads; ++i) {
           const int e = 4 * (l + 32 * i);
-          const float4 u = w && e < dim ? *reinterpret_cast<const float4*>(w + e) : make_float4(1.f, 1.f, 1.f, 1.f);
-          y[i][0] *= inv * u.x;
-          y[i][1] *= inv * u.y;
-          y[i][2] *= inv * u.z;
-          y[i][3] *= inv * u.w;
+          const float4 u = e < dim ? *reinterpret_cast<const float4*>(w + e) : make_float4(1.f, 1.f, 1.f, 1.f);
+          y[i][0] *= inv[b] * u.x;
+          y[i][1] *= inv[b] * u.y;
+          y[i][2] *= inv[b] * u.z;
+          y[i][3] *= inv[b] * u.w;
         }
       }
       if constexpr (kPartner == kExchange) {
@@ -185,15 +207,21 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
   }
 }
 
-template <typename T, int kLanes, int kQuads>
+template <typename T, int kLanes, int kQuads, bool kNorms>
 auto append_kernel(Partner partner) {
   switch (partner) {
-    case kSameQuad: return rope_append_kernel<T, kLanes, kQuads, kSameQuad>;
-    case kOtherLane: return rope_append_kernel<T, kLanes, kQuads, kOtherLane>;
+    case kSameQuad: return rope_append_kernel<T, kLanes, kQuads, kSameQuad, kNorms>;
+    case kOtherLane: return rope_append_kernel<T, kLanes, kQuads, kOtherLane, kNorms>;
     case kOtherQuad:
-      if constexpr (kQuads == 2) return rope_append_kernel<T, kLanes, kQuads, kOtherQuad>;
-    default: return rope_append_kernel<T, kLanes, kQuads, kExchange>;
+      if constexpr (kQuads == 2) return rope_append_kernel<T, kLanes, kQuads, kOtherQuad, kNorms>;
+    default: return rope_append_kernel<T, kLanes, kQuads, kExchange, kNorms>;
   }
+}
+template <typename T, bool kNorms>
+auto append_kernel(int dim, Partner partner) {
+  return dim <= 64    ? append_kernel<T, 16, 1, kNorms>(partner)
+         : dim <= 128 ? append_kernel<T, 32, 1, kNorms>(partner)
+                      : append_kernel<T, 32, 2, kNorms>(partner);
 }
 
 template <typename T>
@@ -206,9 +234,8 @@ int launch_append(const mli_rope_op& op, const mli_kv_cache& cache, int layer, c
                           : half % 4 == 0 && half <= 64     ? kOtherLane
                           : half == 128                     ? kOtherQuad
                                                             : kExchange;
-  const auto kernel = dim <= 64    ? append_kernel<T, 16, 1>(partner)
-                      : dim <= 128 ? append_kernel<T, 32, 1>(partner)
-                                   : append_kernel<T, 32, 2>(partner);
+  // (a kernel without the norms' code moves 4096 tokens of 32 / 8 heads of 128 in 33.7 us, one with it in 34.7)
+  const auto kernel = op.q_norm || op.k_norm ? append_kernel<T, true>(dim, partner) : append_kernel<T, false>(dim, partner);
   // Few tokens: their heads over as many CTAs as put eight on an SM, of four turns a warp at least (500 tokens of 32 / 8
   // heads of 128 with norms 7.9 us, with four on an SM 11.0; 64 tokens 4.0 us, with one turn a warp 5.9).
   const int turn = kAppendWarps * (dim <= 64 ? 2 : 1), heads = op.heads + 2 * cache.kv_heads;
