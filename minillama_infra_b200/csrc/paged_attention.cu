@@ -30,10 +30,10 @@
 // another, data not in L2:
 //   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         95 us   5.63 TB/s
 //   64 rows of 0..8192 tokens, same heads                     174 us   6.13 TB/s
-//   64 rows of 4096, 64 / 8 heads of 128, bf16                176 us   6.12 TB/s
-//   32 rows of 4096, 32 / 4 heads of 256, bf16                115 us   4.69 TB/s
-//   64 rows of 2048, 32 / 8 heads of 128, fp32                169 us   6.36 TB/s
-//   64 rows of 2048, 64 / 8 heads of 128, fp32                237 us   4.54 TB/s
+//   64 rows of 4096, 64 / 8 heads of 128, bf16                178 us   6.05 TB/s
+//   32 rows of 4096, 32 / 4 heads of 256, bf16                114 us   4.73 TB/s
+//   64 rows of 2048, 32 / 8 heads of 128, fp32                174 us   6.17 TB/s
+//   64 rows of 2048, 64 / 8 heads of 128, fp32                227 us   4.76 TB/s
 //   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.64 TB/s
 //   1 row of 53, 32 / 8 heads of 64, fp32                       7 us
 // Equal shares do not end at once (63 to 89 us for the first line: SMs get unequal bandwidth), and
