@@ -156,10 +156,12 @@ class PagedKvCache:
             ops.kv_copy_pages(self.cache, both[0], both[1])
 
     def _upload(self, seqs) -> None:
+        """The rows of seqs, in one copy; entries behind a row's pages are -1."""
         import torch
 
-        for seq in seqs:
-            pages = self._pages[seq]
-            if pages:
-                self.page_table[seq, :len(pages)] = torch.tensor(pages, dtype=torch.int32,
-                                                                 device=self.page_table.device)
+        seqs = sorted(seqs)
+        width = max((len(self._pages[s]) for s in seqs), default=0)
+        if width:
+            rows = [[s, *self._pages[s], *[-1] * (width - len(self._pages[s]))] for s in seqs]
+            new = torch.tensor(rows, dtype=torch.int32, device=self.page_table.device)
+            self.page_table[new[:, 0].long(), :width] = new[:, 1:]

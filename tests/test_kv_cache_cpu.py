@@ -249,6 +249,7 @@ class Checked:
         for s, want in self.want.items():
             assert kv.length(s) == len(want) and len(kv.pages(s)) == -(-len(want) // kv.page_size)
             assert kv.page_table[s, :len(kv.pages(s))].tolist() == kv.pages(s)
+            assert (kv.page_table[s, len(kv.pages(s)):] == -1).all()
             for t, x in enumerate(want):
                 page = kv.pages(s)[t // kv.page_size]
                 assert (kv.cache.k[:, page, :, t % kv.page_size] == x).all()
