@@ -104,6 +104,19 @@ __device__ __forceinline__ unsigned arrive(unsigned* p, unsigned most) {
   return old;
 }
 
+// Reads of another CTA's part from L2.
+__device__ __forceinline__ float read_l2(const float* p) {
+  float x;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 read_l2_4(const float* p) {
+  float4 x;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p)
+               : "memory");
+  return x;
+}
+
 struct Args {
   const float* q;
   float* out;
@@ -131,7 +144,7 @@ struct Piece {
 };
 // What a piece of maximum m counts beside one of maximum top (no piece: 1, and its sums are zero).
 __device__ __forceinline__ float piece_weight(float m, float top, float c) {
-  return m == top ? 1.f : exp2_approx((m - top) * c);
+  return exp2_approx(m == top ? 0.f : (m - top) * c);
 }
 
 // ---- the products on the tensor cores, 16-bit caches --------------------------
@@ -1009,18 +1022,19 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     for (unsigned rest = members; rest;) {  // four at a time
       float w[4], l[4];
       float4 v[4];
-      const int count = __popc(rest);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const Part& x = *piece_at(rest ? __ffs(rest) - 1 : from);
+        const bool on = rest != 0;
+        const Part& x = *piece_at(on ? __ffs(rest) - 1 : from);
         w[u] = x.weight[h];
         l[u] = x.l[h];
         v[u] = *reinterpret_cast<const float4*>(&x.o[h][e]);
+        // one too many adds nothing, and no NaN
+        if (!on) w[u] = l[u] = v[u].x = v[u].y = v[u].z = v[u].w = 0.f;
         rest &= rest - 1;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (u >= count) continue;
         sum_l = fmaf(w[u], l[u], sum_l);
         y = make_float4(fmaf(w[u], v[u].x, y.x), fmaf(w[u], v[u].y, y.y), fmaf(w[u], v[u].z, y.z),
                         fmaf(w[u], v[u].w, y.w));
@@ -1074,23 +1088,31 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
     // slot 0 of all CTAs but the first, in which the segment may be the last one
     const Part* other = parts + 2 * first_cta;
     const Part* first_part = other + (g.start > shares.begin(first_cta) ? 1 : 0);
-    const float c = __ldcg(&first_part->c[h]);
+    const float c = read_l2(&first_part->c[h]);
     float top = -INFINITY, sum_l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 8;  // parts read at once
-    for (int j0 = 0; j0 < count; j0 += kBatch) {
+    int done = 0;
+    const auto join = [&](auto batch) {  // parts whose reads are under way at once
+      constexpr int kBatch = decltype(batch)::value;
       float m[kBatch], l[kBatch];
       float4 v[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const Part* x = j0 + j == 0 ? first_part : other + 2 * min(j0 + j, count - 1);
-        m[j] = __ldcg(&x->m[h]);
-        l[j] = __ldcg(&x->l[h]);
-        v[j] = __ldcg(reinterpret_cast<const float4*>(&x->o[h][e]));
+        const Part* x = done + j == 0 ? first_part : other + 2 * min(done + j, count - 1);
+        m[j] = read_l2(&x->m[h]);
+        l[j] = read_l2(&x->l[h]);
+        v[j] = read_l2_4(&x->o[h][e]);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        if (j0 + j >= count) break;
+        // one too many adds nothing, and no NaN; without a branch, behind which its reads would be moved
+        const bool on = done + j < count;
+        m[j] = on ? m[j] : -INFINITY;
+        l[j] = on ? l[j] : 0.f;
+        v[j] = make_float4(on ? v[j].x : 0.f, on ? v[j].y : 0.f, on ? v[j].z : 0.f, on ? v[j].w : 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
         const float both = fmaxf(top, m[j]);
         const float keep = piece_weight(top, both, c), w = piece_weight(m[j], both, c);
         top = both;
@@ -1098,6 +1120,13 @@ __global__ void __launch_bounds__(kWarpsOf<Math> * 32, 1) paged_attention_kernel
         y = make_float4(fmaf(y.x, keep, w * v[j].x), fmaf(y.y, keep, w * v[j].y), fmaf(y.z, keep, w * v[j].z),
                         fmaf(y.w, keep, w * v[j].w));
       }
+      done += kBatch;
+    };
+    while (done < count) {
+      if (count - done > 4)
+        join(std::integral_constant<int, 16>());
+      else
+        join(std::integral_constant<int, 4>());
     }
     const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
     *reinterpret_cast<float4*>(out_of(g) + h * dim + e) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
