@@ -28,18 +28,18 @@
 // Bound by HBM: 4 products a 16-bit value read with 4 query heads a key-value
 // head.  Measured on one B200 whose copies run at 6.48 TB/s, calls captured one after
 // another, data not in L2:
-//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         95 us   5.63 TB/s
-//   64 rows of 0..8192 tokens, same heads                     174 us   6.13 TB/s
-//   64 rows of 4096, 64 / 8 heads of 128, bf16                178 us   6.05 TB/s
-//   32 rows of 4096, 32 / 4 heads of 256, bf16                114 us   4.73 TB/s
-//   64 rows of 2048, 32 / 8 heads of 128, fp32                174 us   6.17 TB/s
-//   64 rows of 2048, 64 / 8 heads of 128, fp32                227 us   4.76 TB/s
-//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.64 TB/s
-//   1 row of 53, 32 / 8 heads of 64, fp32                       7 us
-// Equal shares do not end at once (63 to 89 us for the first line: SMs get unequal bandwidth), and
-// a call's first bytes are asked for after 2.5 us (lengths, the search of each warp's
-// place, the page table: one after another), its joins take 1.5 to 4 us.  Eight heads of 256, and
-// of fp32, have fewer warps: their queries and pieces take the shared memory.
+//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         91 us   5.92 TB/s
+//   64 rows of 0..8192 tokens, same heads                     173 us   6.19 TB/s
+//   64 rows of 4096, 64 / 8 heads of 128, bf16                174 us   6.18 TB/s
+//   32 rows of 4096, 32 / 4 heads of 256, bf16                113 us   4.75 TB/s
+//   64 rows of 2048, 32 / 8 heads of 128, fp32                172 us   6.26 TB/s
+//   64 rows of 2048, 64 / 8 heads of 128, fp32                227 us   4.75 TB/s
+//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               18 us   3.73 TB/s
+//   1 row of 53, 32 / 8 heads of 64, fp32                       6 us
+// A call's first bytes are asked for after 2 us (lengths, the search of each warp's place, the page
+// table: one after another), its joins take 1 to 3 us; equal shares do not end at once (63 to 89 us for the
+// first line: SMs get unequal bandwidth).  Eight heads of 256, and of fp32, have fewer warps: their queries
+// and pieces take the shared memory.
 #include <float.h>
 #include <math.h>
 
