@@ -32,7 +32,8 @@ class PagedKvCache:
 
         if layout not in ("heads", "tokens"):
             raise ValueError("layout: heads or tokens")
-        if min(layers, pages, kv_heads, head_dim, page_size, max_seqs) <= 0:
+        max_pages = pages if max_pages is None else max_pages
+        if min(layers, pages, kv_heads, head_dim, page_size, max_seqs, max_pages) <= 0:
             raise ValueError("sizes have to be positive")
         dtype = torch.bfloat16 if dtype is None else dtype
         inner = (kv_heads, page_size) if layout == "heads" else (page_size, kv_heads)
@@ -40,7 +41,7 @@ class PagedKvCache:
         if layout == "tokens":
             k, v = k.transpose(2, 3), v.transpose(2, 3)
         self.cache = ops.KvCache(k, v)
-        self.page_size, self.max_pages = page_size, pages if max_pages is None else max_pages
+        self.page_size, self.max_pages = page_size, max_pages
         # -1 names no page: a kernel that is led there reports it
         self.page_table = torch.full((max_seqs, self.max_pages), -1, dtype=torch.int32, device=device)
         self._free_pages = list(range(pages - 1, -1, -1))
@@ -106,8 +107,9 @@ class PagedKvCache:
 
     def fork(self, seq: int) -> int:
         """A new sequence that starts with all of seq's tokens and shares its pages."""
+        pages, length = list(self._pages[seq]), self._lengths[seq]  # before seq's number can be the new one's
         new = self.new()
-        self._pages[new], self._lengths[new] = list(self._pages[seq]), self._lengths[seq]
+        self._pages[new], self._lengths[new] = pages, length
         for page in self._pages[new]:
             self._holders[page] += 1
         self._upload([new])

@@ -336,3 +336,21 @@ def test_pages_run_out_without_a_trace(pool):
     with pytest.raises(ValueError):
         pool(pages=0)
     c.check()
+
+
+def test_unknown_sequences_are_refused_without_a_trace(pool):
+    c = Checked(pool(max_seqs=3))
+    a, b = c.kv.new(), c.kv.new()
+    c.want = {a: []}
+    c.extend([a], [3])
+    c.kv.free(b)
+    for unknown in (b, 7):  # b's row is the one that a fork would take
+        for call in (c.kv.fork, c.kv.free, c.kv.length, c.kv.pages, lambda s: c.kv.extend([a, s])):
+            with pytest.raises(KeyError):
+                call(unknown)
+    c.check()
+    for _ in range(2):  # both rows are still to be had
+        c.want[c.kv.new()] = []
+    c.check()
+    with pytest.raises(ValueError):
+        pool(max_pages=0)
