@@ -465,7 +465,9 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
  * page-table row seq[r] (NULL: row r), so several rows may be tokens of one
  * sequence (a prompt chunk: lengths pos + 1).  Sums and statistics are fp32,
  * and q and p enter the products with all their fp32 bits whatever the cache's
- * type; they and live keys and values are finite (a head with others among them
+ * type, down to 2^-39 (fp16 caches) or 2^-133 (bf16) of the head's largest |q|
+ * and 2^-40 or 2^-134 of its largest weight; q . k is summed before it meets
+ * scale.  They and live keys and values are finite (a head with others among them
  * has outputs that are not).  Slots behind a row's length are not read.  A row of length <= 0 is
  * zero.  A length beyond the page table is cut to it, keys of a page outside
  * the cache are left out, and a row whose seq lies outside the table is zero;

@@ -154,8 +154,9 @@ __device__ __forceinline__ float piece_weight(float m, float top, float c) {
 // each in bf16, 11 in fp16), and the rows of the left operand that a decode
 // step would leave empty carry the parts: rows 0-7 the first of 8 heads, 8-15
 // the second, and a second product the third.  With up to 4 heads rows 0-3, 8-11
-// and 12-15 take all three in one product (128 -> 64 products a tile of 32 tokens of 128).  fp16's range is kept
-// by powers of two: q scaled so that its largest value has exponent 14, p by 2^15.
+// and 12-15 take all three in one product (128 -> 64 products a tile of 32 tokens of 128).  Powers of two keep the parts
+// in range: a head's q is scaled so that its largest value has exponent 14 (fp16) or 0 (bf16), p in fp16 by 2^15.  What the
+// third part cannot hold then lies below 2^-39 or 2^-133 of the largest query, and 2^-40 or 2^-134 of the largest weight.
 // The tensor pipe is busy a fifth of the time: the fifth-generation instruction's 128-row tiles would hold at most 8
 // queries here, and have the values' tile transposed.
 template <typename T>
@@ -238,6 +239,7 @@ struct TensorMath {
   static constexpr int kScratch = kThirdShared ? kSteps * 64 : 0;
   static constexpr int kReadBytes = kUsed * 2;  // of a token
   static constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;
+  static constexpr int kTop = std::is_same<T, __half>::value ? 14 : 0;
   using Part = Piece<kDim, kHeads>;
 
   unsigned q[kSteps][kFew || kThirdShared ? 4 : 6];
@@ -265,28 +267,27 @@ struct TensorMath {
           x[k][j] = live && e < dim ? *reinterpret_cast<const float2*>(row + e) : make_float2(0.f, 0.f);
         }
     };
-    c = scale;
-    float up = 1.f;
-    if (kUp != 1.f) {
-      float top = 0.f;
+    float top = 0.f;
 #pragma unroll
-      for (int k0 = kSteps - kBatch; k0 >= 0; k0 -= kBatch) {
-        read(k0);
+    for (int k0 = kSteps - kBatch; k0 >= 0; k0 -= kBatch) {
+      read(k0);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
+      for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int exponent = (__float_as_int(top) >> 23) & 255;
-      const int f = exponent == 255 ? 127 : min(127 + 60, 268 - exponent);
-      up = __int_as_float(f << 23);
-      c = fmaxf(c * __int_as_float((254 - f) << 23), FLT_MIN);  // c = 0 would make c s of -inf a NaN
+        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
     }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // A power of two, of exponent f - 127, that takes the largest query to exponent kTop; c is divided by it and stays a
+    // normal number: where that holds f back, what the parts lose changes a score times c by less than 2^-100.
+    const int exponent = (__float_as_int(top) >> 23) & 255;
+    const int f = exponent == 255 ? 127
+                                  : max(1, min(min(254 + kTop - exponent, 253), 126 + (__float_as_int(scale) >> 23)));
+    const float up = __int_as_float(f << 23);
+    c = fminf(scale * __int_as_float((254 - f) << 23), FLT_MAX);
 #pragma unroll
     for (int k0 = 0; k0 < kSteps; k0 += kBatch) {
-      if (k0 > 0 || kUp == 1.f) read(k0);  // the maximum's last batch is the first
+      if (k0 > 0) read(k0);  // the maximum's last batch is the first
 #pragma unroll
       for (int k = 0; k < kBatch; ++k)
 #pragma unroll

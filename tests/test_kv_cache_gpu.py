@@ -702,3 +702,24 @@ def test_refusals_name_the_call():
         ops.kv_copy_pages(c, i32([]), i32([]))
     with pytest.raises(ValueError):
         ops.paged_attention_workspace(c, 1, 7)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("power", [-118, -86, -75, -62, 100, 126])
+@pytest.mark.parametrize("group,dim", [(4, 64), (8, 128), (2, 256)])
+def test_attention_of_queries_of_every_size(group, dim, power, dtype):
+    """Queries from near the least normal number to the largest one, with the scale that makes ordinary scores of them:
+    as exact as any others."""
+    g = gen(30)
+    lengths = [150, 3]
+    c, table, kv = filled(g, lengths, 2, 16, dim, dtype)
+    small = 2.0 ** -10 if power > 0 else 1.0  # keys, so that no score overflows
+    c.k.mul_(small)
+    kv = [(k * small, v) for k, v in kv]
+    q = normal(g, 2, 2 * group, dim).clamp(-3.9, 3.9) * 2.0 ** power
+    if power == 126:
+        q[0, 0, 0] = torch.finfo(F32).max
+    scale = dim ** -0.5 / (2.0 ** power * small)
+    got = attend(c, table, q, i32(lengths), scale)
+    for r, (k, v) in enumerate(kv):
+        check_row(got[r], q[r], k, v, scale, f"row {r}")
