@@ -469,7 +469,7 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
  * and 2^-40 or 2^-134 of its largest weight; q . k is summed before it meets
  * scale.  They and live keys and values are finite (a head with others among them
  * has outputs that are not).  Slots behind a row's length are not read.  A row of length <= 0 is
- * zero.  A length beyond the page table is cut to it, keys of a page outside
+ * zero.  A length beyond the page table, or above 2^31 - 64, is cut to it, keys of a page outside
  * the cache are left out, and a row whose seq lies outside the table is zero;
  * each records device error 6.  rows * kv_heads * (tokens
  * that a page-table row can name / 8) stay below 2e9 (MLI_ERR_UNSUPPORTED at worst).

@@ -54,6 +54,8 @@ constexpr int kGroup = 8;         // query heads that share a pass over a segmen
 constexpr int kSlotBytes = 8192;  // one tile's keys, or its values
 constexpr int kSlots = 3;         // of a warp's ring
 constexpr int kMaxCtas = 160;     // CTAs with partial results in the workspace
+// Of a row, so that the numbers of a last tile's tokens (64 at most), counted on from here, are ints.
+constexpr long long kMaxTokens = (1ll << 31) - 64;
 
 // ---- division of n < 2^31 by a number known at launch ------------------------
 struct FastDiv {
@@ -126,7 +128,7 @@ struct Args {
   const int* page_table;
   long long table_stride;
   int rows, heads, table_rows;
-  long long room;  // tokens a page-table row can name
+  long long room;  // tokens a page-table row can name, kMaxTokens at most
   int group;       // query heads of a key-value head
   int chunks;      // passes of up to kGroup of them
   float scale;     // times log2(e)
@@ -1229,6 +1231,7 @@ int mli_paged_attention(const mli_attention_op* op, const mli_kv_cache* cache, i
   a.heads = op->heads;
   a.table_rows = op->table_rows;
   a.room = static_cast<long long>(op->table_cols) * cache->page_size;
+  if (a.room > kMaxTokens) a.room = kMaxTokens;
   a.group = op->heads / cache->kv_heads;
   a.chunks = (a.group + kGroup - 1) / kGroup;
   a.scale = fminf(fmaxf(op->scale * 1.4426950408889634f, FLT_MIN), FLT_MAX);  // log2(e)

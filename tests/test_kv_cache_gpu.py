@@ -723,3 +723,21 @@ def test_attention_of_queries_of_every_size(group, dim, power, dtype):
     got = attend(c, table, q, i32(lengths), scale)
     for r, (k, v) in enumerate(kv):
         check_row(got[r], q[r], k, v, scale, f"row {r}")
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 8), (F32, 4)])
+def test_a_page_table_that_names_2_to_the_31_tokens(dtype, dim):
+    """Two rows of a table of 2049 columns, all the same page of 2^20 slots.  A length above 2^31 - 64 is cut to that and
+    reported; the row beside it is as ever.  Equal weights, and values of one in the first half of the page, of zero in
+    the second: sums of whole numbers, below 2^24 units in a CTA and so exact; the joins of all CTAs round output and
+    sum once each, so a half comes out to 2 sm_count u and a few for the quotient."""
+    size, sms = 1 << 20, torch.cuda.get_device_properties(0).multi_processor_count
+    c = empty_cache(1, 1, 1, size, dim, dtype, fill=0.0)
+    c.v[0, 0, 0, :size // 2] = 1.0
+    table = torch.zeros(2, 2049, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 1, dim, device="cuda")
+    q[1] = 1.0
+    for length, error in ((2 ** 31 - 64, 0), (2 ** 31 - 63, 6), (2 ** 31 - 1, 6)):
+        got = attend(c, table, q, i32([length, 5]), 0.5)
+        assert ops.device_error() == error
+        assert (got[0] - 0.5).abs().max() <= (2 * sms + 8) * U and (got[1] == 1.0).all()
