@@ -477,7 +477,8 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
  * zeroed once before its first use; every call leaves it ready for the next,
  * of any sizes that need no more bytes.  Calls that share a workspace must not overlap on the
  * GPU.  Results do not change from run to run.  q and out 16-byte aligned, strides
- * multiples of 4 floats; out may be q (same stride). */
+ * multiples of 4 floats; out may be q (same stride, MLI_ERR_INVALID_ARG otherwise), and
+ * overlaps nothing else. */
 typedef struct mli_attention_op {
   int rows, heads;
   float scale;           /* > 0 */

@@ -1215,6 +1215,8 @@ int mli_paged_attention(const mli_attention_op* op, const mli_kv_cache* cache, i
   if (bad != MLI_OK || !aligned_rows(op->q, op->q_stride) || !aligned_rows(op->out, op->out_stride) ||
       !aligned(op->workspace, 16))
     return set_status(MLI_ERR_UNSUPPORTED);
+  // in place with another stride, a row's output would land on queries that others still read
+  if (op->out == op->q && op->out_stride != op->q_stride && op->rows > 1) return set_status(MLI_ERR_INVALID_ARG);
   if (op->workspace_bytes <
       mli_paged_attention_workspace_bytes(op->rows, op->heads, cache->kv_heads, cache->head_dim))
     return set_status(MLI_ERR_INVALID_ARG);

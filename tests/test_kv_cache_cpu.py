@@ -354,3 +354,8 @@ def test_unknown_sequences_are_refused_without_a_trace(pool):
     c.check()
     with pytest.raises(ValueError):
         pool(max_pages=0)
+
+
+def test_attention_in_place_takes_one_stride():
+    for change in (dict(out_stride=516), dict(q_stride=516), dict(q_stride=1024, rows=2)):
+        assert _lib.lib().mli_paged_attention(attention(**change), cache(), 0, None) == INVALID
