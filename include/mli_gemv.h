@@ -397,8 +397,9 @@ int mli_argmax(const float* x, int n, long long* out, void* stream);
  * and v, so pages may be laid out head by head, token by token, or with keys
  * and values of a page side by side.  k and v 16-byte aligned, strides and
  * head_dim multiples of 16 bytes, head_dim <= 256 (MLI_ERR_UNSUPPORTED
- * otherwise); elements must not overlap.  The struct itself is read on the
- * host during the call. */
+ * otherwise); elements must not overlap (a stride below head_dim over more than
+ * one entry is MLI_ERR_INVALID_ARG).  The struct itself is read on the host
+ * during the call. */
 typedef struct mli_kv_cache {
   void* k;
   void* v;

@@ -52,6 +52,10 @@ inline int check_cache(const mli_kv_cache* c) {
   if (c->head_dim > kMaxHeadDim || c->head_dim % vec || c->layer_stride % vec || c->page_stride % vec ||
       c->head_stride % vec || c->slot_stride % vec || !aligned(c->k, 16) || !aligned(c->v, 16))
     return MLI_ERR_UNSUPPORTED;
+  // heads that lie on one another (an expanded tensor's): tokens written at once would race
+  if ((c->layers > 1 && c->layer_stride < c->head_dim) || (c->pages > 1 && c->page_stride < c->head_dim) ||
+      (c->kv_heads > 1 && c->head_stride < c->head_dim) || (c->page_size > 1 && c->slot_stride < c->head_dim))
+    return MLI_ERR_INVALID_ARG;
   return MLI_OK;
 }
 

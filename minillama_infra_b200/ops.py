@@ -345,6 +345,8 @@ class KvCache:
         strides = [0 if n == 1 else s for n, s in zip(k.shape, k.stride())]
         if strides != [0 if n == 1 else s for n, s in zip(v.shape, v.stride())] or strides[4] > 1:
             raise ValueError("expected k and v of the same strides, the last dimension contiguous")
+        if any(n > 1 and s < k.shape[4] for n, s in zip(k.shape[:4], strides)):
+            raise ValueError("expected every head of a slot in memory of its own, not an expanded tensor")
         self.k, self.v = k, v
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.get_device()  # -1: host memory, which no kernel takes

@@ -359,3 +359,22 @@ def test_unknown_sequences_are_refused_without_a_trace(pool):
 def test_attention_in_place_takes_one_stride():
     for change in (dict(out_stride=516), dict(q_stride=516), dict(q_stride=1024, rows=2)):
         assert _lib.lib().mli_paged_attention(attention(**change), cache(), 0, None) == INVALID
+
+
+def test_caches_whose_heads_lie_on_one_another_are_refused():
+    l = _lib.lib()
+    for change in (dict(slot_stride=0), dict(slot_stride=56), dict(head_stride=0), dict(page_stride=32),
+                   dict(layer_stride=0), dict(layers=1, layer_stride=0, page_stride=0)):
+        c = cache(**change)
+        assert l.mli_rope_append(rope(), c, 0, None) == INVALID
+        assert l.mli_paged_attention(attention(), c, 0, None) == INVALID
+        assert l.mli_kv_copy_pages(c, A, A, 1, None) == INVALID
+    one = torch.zeros(1, 1, 1, 16, 64)
+    for n in ((2, 1, 1), (1, 2, 1), (1, 1, 2)):
+        t = one.expand(*n, 16, 64)
+        with pytest.raises(ValueError, match="memory of its own"):
+            ops.KvCache(t, t)
+    t = torch.zeros(1, 2, 4, 17 * 32 + 32).as_strided((1, 2, 4, 16, 64), (0, 2304, 576, 32, 1))  # rows of 64, 32 apart
+    with pytest.raises(ValueError, match="memory of its own"):
+        ops.KvCache(t, t)
+    ops.KvCache(one.expand(1, 1, 1, 16, 64), one)  # a stride of 0 over one entry is none
