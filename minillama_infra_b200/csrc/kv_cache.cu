@@ -87,12 +87,16 @@ __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const m
   if (slot < 0 && threadIdx.x == 0 && blockIdx.y == 0) record_device_error(kDevPageRange);
 
   for (int i = threadIdx.x; i < half; i += kAppendThreads) {
-    // the angle's whole turns are dropped in 64 bits: 2^31 positions leave 22 bits of a turn's fraction
-    const double turn = pos * op.turns[i];
+    // pos * turns in two numbers, its whole turns dropped in 64 bits: far positions lose nothing.  The half turns that are
+    // left go to sincospi in fp32; what fp32 does not hold of them (up to pi 2^-25 as an angle: many units of a cosine or
+    // sine near zero) turns its results by that much more.
+    const double turn = __dmul_rn(pos, op.turns[i]), rest = fma(static_cast<double>(pos), op.turns[i], -turn);
+    const double angle = 2.0 * (turn - rint(turn) + rest);
+    const float near = static_cast<float>(angle), more = static_cast<float>(3.14159265358979324 * (angle - near));
     float s, co;
-    sincospif(static_cast<float>(2.0 * (turn - rint(turn))), &s, &co);
-    s_cos[i] = op.amplitude * co;
-    s_sin[i] = op.amplitude * s;
+    sincospif(near, &s, &co);
+    s_cos[i] = op.amplitude * fmaf(-more, s, co);
+    s_sin[i] = op.amplitude * fmaf(more, co, s);
   }
   __syncthreads();
   // a value y of a pair becomes y cs + (the other) sn; values behind rot_dim: y 1 + 0 0

@@ -741,3 +741,38 @@ def test_a_page_table_that_names_2_to_the_31_tokens(dtype, dim):
         got = attend(c, table, q, i32([length, 5]), 0.5)
         assert ops.device_error() == error
         assert (got[0] - 0.5).abs().max() <= (2 * sms + 8) * U and (got[1] == 1.0).all()
+
+
+@pytest.mark.parametrize("first", [0, 131072 - 2000, 2 ** 31 - 2000])
+@pytest.mark.parametrize("amplitude", [1.0, 1.25])
+def test_cosines_and_sines_are_exact_to_their_last_bits(first, amplitude):
+    """Pairs (1, 0) become (cos, sin) of the angle, held against the angle taken from pos * turns in whole numbers.
+    sincospi is off by a unit in the last place (2 u), twice over where the angle's rest that fp32 does not hold cancels
+    half of it; that rest's own roundings (3 u) and the sum's (u) follow, and the amplitude's (u): below 12 u of the value
+    itself, however near a quarter turn the angle is, and the angle itself is held to 2^-53 of a half turn."""
+    g = gen(32)
+    m, dim = 1999, 64
+    pos = torch.arange(first, first + m, device="cuda", dtype=torch.int32)
+    turns = ops.rope_turns(dim)
+    turns[0], turns[1] = 0.25, 0.25 + 2.0 ** -40  # exact quarters, and next to them
+    q = torch.zeros(m, 1, dim, device="cuda")
+    q[..., 0::2] = 1.0
+    c = empty_cache(1, 1, 1, 1, dim, F32)
+    out, kv = torch.empty_like(q), normal(g, m, 1, dim)
+    table = torch.full((1, 1), -1, dtype=torch.int32, device="cuda")  # only the queries are looked at
+    ops.rope_append(out, q, kv, kv, c, 0, pos, table, turns, seq=i32([0] * m), interleaved=True, amplitude=amplitude)
+    assert ops.device_error() == 6
+    got = out[:, 0].double().cpu().numpy().reshape(m, dim // 2, 2)
+    want = np.empty_like(got)
+    for i, t in enumerate(turns.tolist()):
+        num, den = t.as_integer_ratio()
+        for j in range(m):
+            # the angle less its nearest quarter turn, in whole numbers: num / (4 den) turns
+            part = 4 * (first + j) * num
+            quarter = (2 * part + den) // (2 * den)
+            x = 2 * math.pi * ((part - quarter * den) / den) / 4
+            co, si = math.cos(x), math.sin(x)
+            want[j, i] = ((co, si), (-si, co), (-co, -si), (si, -co))[quarter % 4]
+    want *= amplitude
+    err = np.abs(got - want)
+    assert (err <= 12 * U * np.abs(want) + 2.0 ** -50).all(), (err / (12 * U * np.abs(want) + 2.0 ** -50)).max()
