@@ -776,3 +776,20 @@ def test_cosines_and_sines_are_exact_to_their_last_bits(first, amplitude):
     want *= amplitude
     err = np.abs(got - want)
     assert (err <= 12 * U * np.abs(want) + 2.0 ** -50).all(), (err / (12 * U * np.abs(want) + 2.0 ** -50)).max()
+
+
+@pytest.mark.parametrize("dim,tokens,tile,side", [(64, 8192, 32, 2), (128, 4096, 16, 1), (256, 4096, 8, 1)])
+@pytest.mark.parametrize("group", [1, 5])
+def test_fp32_outputs_are_summed_tile_by_tile(dim, tokens, tile, side, group):
+    """Equal weights and equal values, whose running fp32 sum would lose the same half step with every token from 2048
+    on: as many rows as there are warps, so that each sums a row alone.  A tile's sum takes tile / side roundings, the
+    sum of the tiles one each, lanes, quotient and product four: each at most u of a sum of positive numbers."""
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    value = 1 + 2.0 ** -13 - 2.0 ** -20
+    c = empty_cache(1, tokens // 64, 1, 64, dim, F32, fill=value)
+    table = torch.arange(tokens // 64, device="cuda", dtype=torch.int32)[None]
+    q = torch.zeros(rows, group, dim, device="cuda")
+    got = attend(c, table, q, i32([tokens] * rows), 0.125, seq=i32([0] * rows))
+    value = float(c.v[0, 0, 0, 0, 0])
+    err = (got.double() - value).abs().max().item()
+    assert err <= (tile / side + tokens / tile + 4) * U * value, err / (U * value)
