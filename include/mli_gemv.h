@@ -468,12 +468,15 @@ int mli_rope_append(const mli_rope_op* op, const mli_kv_cache* cache, int layer,
  * and q and p enter the products with all their fp32 bits whatever the cache's
  * type, down to 2^-39 (fp16 caches) or 2^-133 (bf16) of the head's largest |q|
  * and 2^-40 or 2^-134 of its largest weight; q . k is summed before it meets
- * scale.  They and live keys and values are finite (a head with others among them
- * has outputs that are not).  Slots behind a row's length are not read.  A row of length <= 0 is
+ * scale.  They and live keys and values are finite.  A head with others among them
+ * has outputs that are not, but for a key whose score comes out as -inf: that
+ * weighs nothing, and the head's outputs are those of its other tokens.  Slots
+ * behind a row's length are not read.  A row of length <= 0 is
  * zero.  A length beyond the page table, or above 2^31 - 64, is cut to it, keys of a page outside
  * the cache are left out, and a row whose seq lies outside the table is zero;
- * each records device error 6.  rows * kv_heads * (tokens
- * that a page-table row can name / 8) stay below 2e9 (MLI_ERR_UNSUPPORTED at worst).
+ * each records device error 6.  With g = heads / kv_heads, rows * kv_heads *
+ * ceil(g / 8) * (tokens that a page-table row can name / 8) up to 2e9 are taken,
+ * more may be MLI_ERR_UNSUPPORTED.
  * `workspace`: mli_paged_attention_workspace_bytes bytes of device memory, 16-byte aligned,
  * zeroed once before its first use; every call leaves it ready for the next,
  * of any sizes that need no more bytes.  Calls that share a workspace must not overlap on the

@@ -378,3 +378,13 @@ def test_caches_whose_heads_lie_on_one_another_are_refused():
     with pytest.raises(ValueError, match="memory of its own"):
         ops.KvCache(t, t)
     ops.KvCache(one.expand(1, 1, 1, 16, 64), one)  # a stride of 0 over one entry is none
+
+
+def test_tiles_are_counted_once_for_every_eight_heads():
+    """rows * kv_heads * ceil(group / 8) * (tokens / 8) of an fp32 cache of 256 dims, whose tiles are the smallest."""
+    c = cache(dtype=0, head_dim=256, layer_stride=8 * 4 * 16 * 256, page_stride=4 * 16 * 256, head_stride=16 * 256,
+              slot_stride=256)
+    wide = dict(rows=256, q_stride=128 * 256, out_stride=128 * 256, q=2 * A, table_cols=948000, table_stride=948000)
+    assert 256 * 4 * (948000 * 16 // 8) < 2e9 < 256 * 4 * 2 * (948000 * 16 // 8)
+    for heads in (36, 64, 128):  # groups of 9, 16 and 32: two passes and four
+        assert _lib.lib().mli_paged_attention(attention(heads=heads, **wide), c, 0, None) == UNSUPPORTED

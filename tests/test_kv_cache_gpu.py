@@ -793,3 +793,27 @@ def test_fp32_outputs_are_summed_tile_by_tile(dim, tokens, tile, side, group):
     value = float(c.v[0, 0, 0, 0, 0])
     err = (got.double() - value).abs().max().item()
     assert err <= (tile / side + tokens / tile + 4) * U * value, err / (U * value)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_an_infinite_key_makes_a_head_not_finite_or_leaves_its_token_out(dtype):
+    """A score of -inf weighs nothing, one of inf or NaN reaches every output of its head: with an fp32 cache by the
+    query's sign, with the others by what the parts of the query multiply it to."""
+    g = gen(31)
+    lengths = [100] * 4
+    c, table, kv = filled(g, lengths, 2, 16, 64, dtype)
+    q = normal(g, 4, 4, 64)
+    for r, x in enumerate((math.inf, math.inf, -math.inf, -math.inf)):
+        c.k[0, table[r, 3].long(), 0, 2, 5] = x  # token 50
+        q[r, :2, 5] = q[r, :2, 5].abs() * (1 if r % 2 else -1)
+    got = attend(c, table, q, i32(lengths), 0.125)
+    rest = [t for t in range(100) if t != 50]
+    for r in range(4):
+        below = (r % 2 == 0) == (r < 2)  # the scores are -inf
+        for h in range(2):
+            if dtype == F32 or not got[r, h].isfinite().any():
+                assert got[r, h].isfinite().all() if dtype == F32 and below else got[r, h].isnan().all()
+            if got[r, h].isfinite().any():
+                assert below
+                check_row(got[r, h:h + 1], q[r, h:h + 1], kv[r][0][rest, :1], kv[r][1][rest, :1], 0.125)
+        check_row(got[r, 2:], q[r, 2:], kv[r][0][:, 1:], kv[r][1][:, 1:], 0.125)
