@@ -70,7 +70,8 @@ class PagedKvCache:
 
     def extend(self, seqs, counts=None) -> None:
         """Slots for counts[i] (one) more tokens of seqs[i].  All or nothing: without
-        pages enough, MemoryError, and nothing has changed."""
+        pages enough, MemoryError, and nothing has changed; nor has it when a copy
+        or an update of the page table raises (every method keeps to that)."""
         seqs = list(seqs)
         counts = [1] * len(seqs) if counts is None else list(counts)
         if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(n < 0 for n in counts):
@@ -90,40 +91,51 @@ class PagedKvCache:
                 needed += 1
         if needed > len(self._free_pages):
             raise MemoryError(f"{needed} pages needed, {len(self._free_pages)} free")
-        moved = []
+        # the device first: should it refuse, the pages are still free and the sequences what they were
+        taken = self._free_pages[len(self._free_pages) - needed:]
+        free, moved, new = list(taken), [], {}
         for seq in copies:
-            old, page = self._pages[seq][-1], self._take()
-            self._holders[old] -= 1
-            self._pages[seq][-1] = page
+            old, page = self._pages[seq][-1], free.pop()
             moved.append((old, page))
-        changed = set(copies)
+            new[seq] = [*self._pages[seq][:-1], page]
+        for seq, n in zip(seqs, counts):
+            more = -(-(self._lengths[seq] + n) // self.page_size) - len(self._pages[seq])
+            if more:
+                new[seq] = [*new.get(seq, self._pages[seq]), *(free.pop() for _ in range(more))]
+        self._copy(moved)
+        self._upload(new)
+        del self._free_pages[len(self._free_pages) - needed:]
+        for page in taken:
+            self._holders[page] = 1
+        for old, _ in moved:
+            self._holders[old] -= 1
+        self._pages.update(new)
         for seq, n in zip(seqs, counts):
             self._lengths[seq] += n
-            while len(self._pages[seq]) * self.page_size < self._lengths[seq]:
-                self._pages[seq].append(self._take())
-                changed.add(seq)
-        self._copy(moved)
-        self._upload(changed)
 
     def fork(self, seq: int) -> int:
         """A new sequence that starts with all of seq's tokens and shares its pages."""
-        pages, length = list(self._pages[seq]), self._lengths[seq]  # before seq's number can be the new one's
-        new = self.new()
+        pages, length = list(self._pages[seq]), self._lengths[seq]  # before a row is looked for
+        if not self._free_rows:
+            raise MemoryError("every row of the page table is in use")
+        new = self._free_rows[-1]
+        self._upload({new: pages})
+        self._free_rows.pop()
         self._pages[new], self._lengths[new] = pages, length
-        for page in self._pages[new]:
+        for page in pages:
             self._holders[page] += 1
-        self._upload([new])
         return new
 
     def free(self, seq: int) -> None:
         """Gives the sequence's row back, and the pages that no other holds."""
-        for page in self._pages.pop(seq):
+        pages = self._pages[seq]
+        self.page_table[seq].fill_(-1)
+        del self._pages[seq], self._lengths[seq]
+        for page in pages:
             self._holders[page] -= 1
             if not self._holders[page]:
                 self._free_pages.append(page)
-        del self._lengths[seq]
         self._free_rows.append(seq)
-        self.page_table[seq].fill_(-1)
 
     def compact(self) -> int:
         """Moves pages so that those in use are the first ones; how many moved."""
@@ -133,22 +145,15 @@ class PagedKvCache:
         moved = dict(zip((p for p in range(used, len(self._holders)) if self._holders[p]), holes))
         if not moved:
             return 0
+        new = {seq: [moved.get(p, p) for p in pages] for seq, pages in self._pages.items()
+               if any(p in moved for p in pages)}
         self._copy(list(moved.items()))
+        self._upload(new)
         for old, page in moved.items():
             self._holders[page], self._holders[old] = self._holders[old], 0
-        changed = []
-        for seq, pages in self._pages.items():
-            if any(p in moved for p in pages):
-                self._pages[seq] = [moved.get(p, p) for p in pages]
-                changed.append(seq)
+        self._pages.update(new)
         self._free_pages = list(range(len(self._holders) - 1, used - 1, -1))
-        self._upload(changed)
         return len(moved)
-
-    def _take(self) -> int:
-        page = self._free_pages.pop()
-        self._holders[page] = 1
-        return page
 
     def _copy(self, pairs) -> None:
         import torch
@@ -157,13 +162,12 @@ class PagedKvCache:
             both = torch.tensor(pairs, dtype=torch.int32, device=self.page_table.device).T.contiguous()
             ops.kv_copy_pages(self.cache, both[0], both[1])
 
-    def _upload(self, seqs) -> None:
-        """The rows of seqs, in one copy; entries behind a row's pages are -1."""
+    def _upload(self, changed) -> None:
+        """The rows of the page table that become changed[row], in one copy; entries behind a row's pages are -1."""
         import torch
 
-        seqs = sorted(seqs)
-        width = max((len(self._pages[s]) for s in seqs), default=0)
+        width = max((len(pages) for pages in changed.values()), default=0)
         if width:
-            rows = [[s, *self._pages[s], *[-1] * (width - len(self._pages[s]))] for s in seqs]
+            rows = [[s, *pages, *[-1] * (width - len(pages))] for s, pages in sorted(changed.items())]
             new = torch.tensor(rows, dtype=torch.int32, device=self.page_table.device)
             self.page_table[new[:, 0].long(), :width] = new[:, 1:]

@@ -388,3 +388,68 @@ def test_tiles_are_counted_once_for_every_eight_heads():
     assert 256 * 4 * (948000 * 16 // 8) < 2e9 < 256 * 4 * 2 * (948000 * 16 // 8)
     for heads in (36, 64, 128):  # groups of 9, 16 and 32: two passes and four
         assert _lib.lib().mli_paged_attention(attention(heads=heads, **wide), c, 0, None) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("broken", ["copy", "upload"])
+def test_device_calls_that_fail_leave_no_trace(pool, monkeypatch, broken):
+    """A page copy or an update of the page table that raises (no memory, a capture under way): the sequences, their
+    pages and the free ones are what they were, and the same call succeeds later."""
+    c = Checked(pool(pages=16))
+
+    def trace():
+        kv = c.kv
+        return (dict(kv._lengths), {s: list(p) for s, p in kv._pages.items()}, list(kv._holders), list(kv._free_pages),
+                list(kv._free_rows), kv.page_table.clone())
+
+    def fails(call, copies=True):
+        before = trace()
+        with monkeypatch.context() as m:
+            def raises(*args, **kw):
+                raise RuntimeError("broken")
+
+            if broken == "copy":
+                m.setattr(ops, "kv_copy_pages", raises)
+            else:
+                m.setattr(c.kv, "page_table", _Unwritable(c.kv.page_table))
+            if broken == "upload" or copies:
+                with pytest.raises(RuntimeError, match="broken"):
+                    call()
+                assert trace()[:5] == before[:5]
+        assert torch.equal(c.kv.page_table, before[5])
+        c.check()
+
+    a, b = c.kv.new(), c.kv.new()
+    c.want = {a: [], b: []}
+    fails(lambda: c.kv.extend([a, b], [6, 9]), copies=False)
+    c.extend([a, b], [6, 9])
+    fails(lambda: c.kv.fork(a), copies=False)
+    d = c.kv.fork(a)
+    c.want[d] = list(c.want[a])
+    fails(lambda: c.kv.extend([a, d, b], [1, 3, 4]))
+    c.extend([a, d, b], [1, 3, 4])
+    c.check()
+    fails(lambda: c.kv.free(b), copies=False)
+    c.kv.free(a)
+    del c.want[a]
+    fails(c.kv.compact)
+    assert c.kv.compact() > 0
+    c.check()
+
+
+class _Unwritable:
+    """A page table that can be read, and whose every write raises."""
+
+    def __init__(self, table):
+        self._table, self.device = table, table.device
+
+    def clone(self):
+        return self._table.clone()
+
+    def __getitem__(self, at):
+        return self
+
+    def __setitem__(self, at, value):
+        raise RuntimeError("broken")
+
+    def fill_(self, value):
+        raise RuntimeError("broken")
