@@ -4,7 +4,9 @@
 the page table; a page may belong to several of them (forks), and is copied for
 one of them when that one is about to write into it.  The bookkeeping is on the
 host; the tensors that the kernels read (`cache`, `page_table`) are on the
-device, and every change of them is ordered on the current stream.
+device, and every change of them is ordered on the current stream (which must
+not be capturing then: RuntimeError).  A token that needs no new page changes
+nothing on the device; one that does sends one entry of the page table.
 
     kv = PagedKvCache(layers=16, pages=4096, kv_heads=8, head_dim=64, max_seqs=64)
     s = kv.new()
@@ -15,6 +17,8 @@ device, and every change of them is ordered on the current stream.
     kv.free(s); kv.compact()
 """
 from __future__ import annotations
+
+from array import array
 
 from . import ops
 
@@ -78,40 +82,45 @@ class PagedKvCache:
             raise ValueError("expected distinct sequences and a count >= 0 for each")
         # how many hold each page, as the copies below change it
         holders = {p: self._holders[p] for s in seqs for p in self._pages[s][-1:]}
-        copies, needed = [], 0
+        copies, more = [], []
         for seq, n in zip(seqs, counts):
             have, length = self._pages[seq], self._lengths[seq]
             want = -(-(length + n) // self.page_size)
             if want > self.max_pages:
                 raise MemoryError(f"sequence {seq}: {length + n} tokens need more than {self.max_pages} pages")
-            needed += want - len(have)
+            more.append(want - len(have))
             if n and length % self.page_size and holders[have[-1]] > 1:
                 holders[have[-1]] -= 1
                 copies.append(seq)
-                needed += 1
+        needed = sum(more) + len(copies)
         if needed > len(self._free_pages):
             raise MemoryError(f"{needed} pages needed, {len(self._free_pages)} free")
-        # the device first: should it refuse, the pages are still free and the sequences what they were
-        taken = self._free_pages[len(self._free_pages) - needed:]
-        free, moved, new = list(taken), [], {}
-        for seq in copies:
-            old, page = self._pages[seq][-1], free.pop()
-            moved.append((old, page))
-            new[seq] = [*self._pages[seq][:-1], page]
-        for seq, n in zip(seqs, counts):
-            more = -(-(self._lengths[seq] + n) // self.page_size) - len(self._pages[seq])
-            if more:
-                new[seq] = [*new.get(seq, self._pages[seq]), *(free.pop() for _ in range(more))]
-        self._copy(moved)
-        self._upload(new)
-        del self._free_pages[len(self._free_pages) - needed:]
-        for page in taken:
-            self._holders[page] = 1
-        for old, _ in moved:
-            self._holders[old] -= 1
-        self._pages.update(new)
+        if needed:
+            self._grow(seqs, copies, more, needed)
         for seq, n in zip(seqs, counts):
             self._lengths[seq] += n
+
+    def _grow(self, seqs, copies, more, needed) -> None:
+        """Copies of the last pages of `copies`, and more[i] new pages for seqs[i]: `needed` in all."""
+        pages = self._free_pages[len(self._free_pages) - needed:][::-1]
+        moved = [(self._pages[seq][-1], page) for seq, page in zip(copies, pages)]
+        rows, cols, at = list(copies), [len(self._pages[seq]) - 1 for seq in copies], len(copies)
+        for seq, n in zip(seqs, more):
+            if n:
+                rows += [seq] * n
+                cols += range(len(self._pages[seq]), len(self._pages[seq]) + n)
+        # the device first: should it refuse, the pages are still free and the sequences what they were
+        self._copy(moved)
+        self._write(rows, cols, pages)
+        del self._free_pages[len(self._free_pages) - needed:]
+        for page in pages:
+            self._holders[page] = 1
+        for seq, (old, page) in zip(copies, moved):
+            self._holders[old] -= 1
+            self._pages[seq][-1] = page
+        for seq, n in zip(seqs, more):
+            self._pages[seq] += pages[at:at + n]
+            at += n
 
     def fork(self, seq: int) -> int:
         """A new sequence that starts with all of seq's tokens and shares its pages."""
@@ -119,7 +128,8 @@ class PagedKvCache:
         if not self._free_rows:
             raise MemoryError("every row of the page table is in use")
         new = self._free_rows[-1]
-        self._upload({new: pages})
+        if pages:
+            self.page_table[new, :len(pages)] = self._send(pages)[0]
         self._free_rows.pop()
         self._pages[new], self._lengths[new] = pages, length
         for page in pages:
@@ -129,6 +139,7 @@ class PagedKvCache:
     def free(self, seq: int) -> None:
         """Gives the sequence's row back, and the pages that no other holds."""
         pages = self._pages[seq]
+        self._check_stream()
         self.page_table[seq].fill_(-1)
         del self._pages[seq], self._lengths[seq]
         for page in pages:
@@ -145,29 +156,48 @@ class PagedKvCache:
         moved = dict(zip((p for p in range(used, len(self._holders)) if self._holders[p]), holes))
         if not moved:
             return 0
-        new = {seq: [moved.get(p, p) for p in pages] for seq, pages in self._pages.items()
-               if any(p in moved for p in pages)}
+        entries = [(seq, col, moved[page]) for seq, pages in self._pages.items() for col, page in enumerate(pages)
+                   if page in moved]
         self._copy(list(moved.items()))
-        self._upload(new)
+        self._write(*zip(*entries))
         for old, page in moved.items():
             self._holders[page], self._holders[old] = self._holders[old], 0
-        self._pages.update(new)
+        for seq, col, page in entries:
+            self._pages[seq][col] = page
         self._free_pages = list(range(len(self._holders) - 1, used - 1, -1))
         return len(moved)
 
+    def _check_stream(self) -> bool:
+        """Whether the cache is a GPU's.  A change within a capture would be made at its replays, not now."""
+        import torch
+
+        on_gpu = self.page_table.device.type == "cuda"
+        if on_gpu and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the pages of a cache cannot change while the current stream is capturing")
+        return on_gpu
+
+    def _send(self, *lists):
+        """Lists of one length as rows of an int32 tensor on the device, by a copy that the host does not wait for."""
+        import torch
+
+        on_gpu = self._check_stream()
+        numbers = array("i")
+        for x in lists:
+            numbers.extend(x)
+        t = torch.frombuffer(numbers, dtype=torch.int32).view(len(lists), -1)
+        return (t.pin_memory() if on_gpu else t).to(self.page_table.device, non_blocking=True)
+
     def _copy(self, pairs) -> None:
-        import torch
-
         if pairs:
-            both = torch.tensor(pairs, dtype=torch.int32, device=self.page_table.device).T.contiguous()
-            ops.kv_copy_pages(self.cache, both[0], both[1])
+            ops.kv_copy_pages(self.cache, *self._send(*zip(*pairs)))
 
-    def _upload(self, changed) -> None:
-        """The rows of the page table that become changed[row], in one copy; entries behind a row's pages are -1."""
-        import torch
-
-        width = max((len(pages) for pages in changed.values()), default=0)
-        if width:
-            rows = [[s, *pages, *[-1] * (width - len(pages))] for s, pages in sorted(changed.items())]
-            new = torch.tensor(rows, dtype=torch.int32, device=self.page_table.device)
-            self.page_table[new[:, 0].long(), :width] = new[:, 1:]
+    def _write(self, rows, cols, pages) -> None:
+        """page_table[rows[i], cols[i]] = pages[i], and no others: a token that crosses into a new page changes one
+        entry, however long its sequence."""
+        if len(rows) <= 4:  # a fill takes 7 us, sending numbers and an indexed write 36
+            self._check_stream()
+            for row, col, page in zip(rows, cols, pages):
+                self.page_table[row, col].fill_(page)
+        else:
+            rows, cols, pages = self._send(rows, cols, pages)
+            self.page_table[rows, cols] = pages

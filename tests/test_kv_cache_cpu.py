@@ -453,3 +453,33 @@ class _Unwritable:
 
     def fill_(self, value):
         raise RuntimeError("broken")
+
+
+@pytest.mark.parametrize("seqs", [1, 2, 7])
+def test_only_entries_that_change_are_written(pool, monkeypatch, seqs):
+    """A token in a new page writes its one entry, a copied page its one; a compaction those of the pages it moved."""
+    c = Checked(pool(pages=200, max_seqs=9))
+    sent, write = [], c.kv._write
+    monkeypatch.setattr(c.kv, "_write", lambda *lists: (sent.append([list(x) for x in lists]), write(*lists))[1])
+    all_, b = [c.kv.new() for _ in range(seqs)], c.kv.new()
+    c.want = {s: [] for s in [*all_, b]}
+    c.extend([b], [7])
+    c.extend(all_, [76] * seqs)
+    sent.clear()
+    c.extend([*all_, b], [1] * seqs + [1])
+    assert sent == [[all_, [19] * seqs, [c.kv.pages(s)[19] for s in all_]]]
+    sent.clear()
+    c.extend([*all_, b], [1] * seqs + [0])
+    assert not sent
+    d = c.kv.fork(all_[0])
+    c.want[d] = list(c.want[all_[0]])
+    c.extend([d], [1])
+    assert sent == [[[d], [19], [c.kv.pages(d)[19]]]]
+    c.kv.free(b)
+    del c.want[b]
+    sent.clear()
+    before = {s: c.kv.pages(s) for s in [*all_, d]}
+    assert c.kv.compact() == 2
+    changed = [(s, i, p) for s in before for i, p in enumerate(c.kv.pages(s)) if p != before[s][i]]
+    assert sorted(zip(*sent[0])) == sorted(changed)
+    c.check()

@@ -817,3 +817,32 @@ def test_an_infinite_key_makes_a_head_not_finite_or_leaves_its_token_out(dtype):
                 assert below
                 check_row(got[r, h:h + 1], q[r, h:h + 1], kv[r][0][rest, :1], kv[r][1][rest, :1], 0.125)
         check_row(got[r, 2:], q[r, 2:], kv[r][0][:, 1:], kv[r][1][:, 1:], 0.125)
+
+
+def test_pages_do_not_change_within_a_capture():
+    """Each of PagedKvCache's changes is refused while the current stream captures, and leaves no trace."""
+    kv = PagedKvCache(layers=1, pages=8, kv_heads=2, head_dim=64, page_size=4, max_seqs=3)
+    a, b = kv.new(), kv.new()
+    kv.extend([a, b], [4, 5])
+    kv.free(a)
+    a = kv.new()
+    x = torch.zeros(4, device="cuda")
+    table = kv.page_table.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: kv.extend([b], [4]), lambda: kv.fork(b), lambda: kv.free(b), kv.compact):
+            with pytest.raises(RuntimeError, match="capturing"):
+                call()
+        kv.extend([b], [3])  # no new page
+        x.add_(1.0)
+    graph.replay()
+    assert (x == 1).all() and torch.equal(kv.page_table, table)
+    assert kv.length(b) == 8 and len(kv.pages(b)) == 2 and kv.free_pages == 6
+    kv.extend([b], [1])
+    c = kv.fork(b)
+    kv.extend([c])  # pages 1, 2 and 3; page 0 is b's third
+    kv.free(b)
+    assert kv.compact() == 1 and sorted(kv.pages(c)) == [0, 1, 2]
+    assert kv.page_table[c, :3].tolist() == kv.pages(c) and (kv.page_table[c, 3:] == -1).all()
+    assert (kv.page_table[[a, b]] == -1).all()
