@@ -12,8 +12,8 @@
 namespace mli {
 namespace {
 
-// Two warps: each repeats a token's set-up, so 8192 tokens of 24 / 8 heads of 128 took 57 us with four and 52 with two;
-// with one (52 us) 1999 tokens of 35 / 5 heads of 80 took 31 us instead of 22.
+// Two warps: each repeats a token's set-up, so 8192 tokens of 24 / 8 heads of 128 take 54 us with four and 51 with two;
+// with one (50 us) 1999 tokens of 35 / 5 heads of 80 take 24 us instead of 18, 500 of 32 / 8 heads of 128 11 instead of 7.
 constexpr int kAppendWarps = 2;
 constexpr int kAppendThreads = kAppendWarps * 32;
 
@@ -39,7 +39,7 @@ __device__ __forceinline__ void store4(T* p, const float (&y)[4]) {
 // its token's cosines and sines (one pair a thread, in shared memory; from there each lane keeps those of its own
 // values for all heads).  blockIdx.x is the token; blockIdx.y shares out the heads of few tokens.
 // 8192 tokens of 24 / 8 heads of 128 into a bf16 cache: 51 us, 5.90 TB/s of 302 MB (copies run at 6.48); 64 tokens with
-// norms 3.9 us, one token 2.7 us.  With norms the instructions bind: 4096 tokens of 32 / 8 heads of 128 38 us, 4.81 TB/s;
+// norms 3.7 us, one token 2.5 us.  With norms the instructions bind: 4096 tokens of 32 / 8 heads of 128 38 us, 4.81 TB/s;
 // 1999 tokens of 35 / 5 heads of 80, 20 of 32 lanes in use, 18 us, 3.0 TB/s.
 template <typename T, int kLanes, int kQuads, Partner kPartner, bool kNorms>
 __global__ void __launch_bounds__(kAppendThreads, 12) rope_append_kernel(const mli_rope_op op, const CacheLayer<T> c) {
@@ -262,7 +262,7 @@ struct CopyArgs {
 };
 
 // One CTA per (pair, layer, keys or values); bound by HBM, reads and writes alike: 256 pages of 16 tokens, 28 layers of
-// 8 heads of 128 in bf16 (470 MB), 144 us, 6.53 TB/s read and written; 4 pages of 16 layers of 8 heads of 64, 2.4 us.
+// 8 heads of 128 in bf16 (470 MB), 143 us, 6.57 TB/s read and written; 4 pages of 16 layers of 8 heads of 64, 2.2 us.
 template <bool kWhole>  // a page is one row
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs a, const int* src, const int* dst) {
   griddep_wait();

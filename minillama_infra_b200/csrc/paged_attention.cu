@@ -23,18 +23,19 @@
 // row permuted by its number so that column reads do not collide); warps never
 // wait for one another before the join.  Slots of 8 KB with three to a warp and
 // eight warps keep up to 192 KB a SM under way; four warps with 16 KB tiles of keys and
-// values together reached 3.4 TB/s where this reaches 5.6.
+// values together reached 3.4 TB/s on the first line below.
 //
 // Bound by HBM: 4 products a 16-bit value read with 4 query heads a key-value
 // head.  Measured on one B200 whose copies run at 6.48 TB/s, calls captured one after
 // another, data not in L2:
-//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         91 us   5.92 TB/s
-//   64 rows of 0..8192 tokens, same heads                     173 us   6.19 TB/s
-//   64 rows of 4096, 64 / 8 heads of 128, bf16                174 us   6.18 TB/s
-//   32 rows of 4096, 32 / 4 heads of 256, bf16                113 us   4.75 TB/s
-//   64 rows of 2048, 32 / 8 heads of 128, fp32                172 us   6.26 TB/s
+//   1 row of 131072 tokens, 24 / 8 heads of 128, bf16         91 us   5.90 TB/s
+//   64 rows of 0..8192 tokens, same heads                     174 us   6.15 TB/s
+//   64 rows of 4096, 64 / 8 heads of 128, bf16                175 us   6.14 TB/s
+//   32 rows of 4096, 32 / 4 heads of 256, bf16                115 us   4.67 TB/s
+//   64 rows of 2048, 32 / 8 heads of 128, fp32                174 us   6.17 TB/s
 //   64 rows of 2048, 64 / 8 heads of 128, fp32                218 us   4.93 TB/s
-//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               18 us   3.73 TB/s
+//   64 rows of 2048, 128 / 8 heads of 128, bf16 (two passes)  168 us   3.20 TB/s of the bytes of one
+//   16 rows of 1..4096, 32 / 8 heads of 64, bf16               19 us   3.69 TB/s
 //   1 row of 53, 32 / 8 heads of 64, fp32                       6 us
 // A call's first bytes are asked for after 2 us (lengths, the search of each warp's place, the page
 // table: one after another), its joins take 1 to 3 us; equal shares do not end at once (63 to 89 us for the
@@ -235,8 +236,9 @@ struct TensorMath {
   static constexpr int kHeads = kFew ? 4 : 8;
   static constexpr int kSteps = kUsed / 16;
   // The third parts of 8 heads' queries of 128 dims and more do not fit in registers beside the rest: they are in shared
-  // memory, which costs a warp (64 rows of 4096, 64 / 8 heads of 128: 178 us, spilling them 180; 32 rows, 32 / 4 heads
-  // of 256: 121 and 215).
+  // memory, which costs a warp (64 rows of 4096, 64 / 8 heads of 128: 175 us, spilling them 181; 32 rows, 32 / 4 heads
+  // of 256: 116 and 130; 256 rows of 100, 64 / 8 heads of 128: 37.7 and 36.4).  The kernels for 256 dims but that of 8 heads
+  // in fp16 still spill 20 bytes.
   static constexpr bool kThirdShared = kUsed >= 128 && !kFew;
   static constexpr int kScratch = kThirdShared ? kSteps * 64 : 0;
   static constexpr int kReadBytes = kUsed * 2;  // of a token
@@ -310,7 +312,9 @@ struct TensorMath {
     for (int i = 0; i < kUsed / 8; ++i) o[i] = make_float2(0.f, 0.f);
   }
 
-  // The tile's weights from its keys.  live: bit t for token t.
+  // The tile's weights from its keys.  live: bit t for token t.  A score runs through 4 to 32 products one after another,
+  // whose fp32 sums the tensor cores truncate.  That is left so: at its worst, values of one sign in 256 dims, a score is
+  // off by 2.1 u of sum |q k| in the root mean square (u = 2^-24), the fp32 product of the plain form by 5.7 u.
   __device__ __forceinline__ void scores(unsigned keys, unsigned long long live, const float* scratch) {
     const int lane = threadIdx.x & 31, mat = lane >> 3, in = lane & 7;
     float s[kTok / 8][4];
@@ -1166,9 +1170,10 @@ int launch_math(const Args& a, const mli_attention_op& op, const mli_kv_cache& c
 
 template <typename T, int kDim, int kUsed>
 int launch_dim(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
-  // half of the products where all heads of a pass fit beside their parts; against the kernel for 8 heads: 256 rows of
-  // 100 tokens, 4 heads of 128, 28.4 and 35.3 us; 32 rows of 4096, 4 of 256, 97 and 117 us; fp32, 16 rows to 1024, 4 of
-  // 64, 14.8 and 18.9 us; 64 rows of 4096, 4 of 128, 176 and 173 us (bound by HBM)
+  // Half of the products where all heads of a pass fit beside their parts.  With the kernel for 4 heads and with the one
+  // for 8, bf16: 256 rows of 100 tokens, 32 / 8 heads of 128, 27.8 and 34.2 us; 64 rows of 2048, 16 / 4 heads of 256, 96
+  // and 111; 16 rows to 4096, 32 / 8 of 64, 18.5 and 20.2; bound by HBM, 64 rows of 4096, 32 / 8 of 128, 175 and 174, of
+  // 2048 92.7 and 91.6.  fp32: 16 rows to 1024, 32 / 8 of 64, 13.3 and 18.1; 64 rows of 2048, 32 / 8 of 128, 174 and 213.
   const bool few = a.group <= 4;
   if constexpr (sizeof(T) == 4)
     return few ? launch_math<FloatMath<kDim, true>, T, kDim>(a, op, cache, layer, s)
@@ -1182,9 +1187,10 @@ template <typename T>
 int launch_attention(const Args& a, const mli_attention_op& op, const mli_kv_cache& cache, int layer, cudaStream_t s) {
   const int dim = cache.head_dim;
   if (dim <= 64) return launch_dim<T, 64, 64>(a, op, cache, layer, s);
-  // the tensor cores' share of a call goes by the dims they multiply: 80 and 96 have kernels of their own
-  // (64 rows of 2048, 64 / 8 heads: 66 and 74 us, with the kernel for 128 90 and 91 us; with 32 / 8 heads, bound by
-  // HBM, 64 us against 68 for 80, 137 against 134 for 96)
+  // The tensor cores' share of a call goes by the dims they multiply: 80 and 96 have kernels of their own.  With them and
+  // with the one for 128, bf16: 64 rows of 2048, 64 / 8 heads, 66 and 88 us of 80, 75 and 89 of 96; 256 rows of 100, 32 / 8
+  // heads, 23.6 and 26.0 of 80, 25.2 and 26.6 of 96; bound by HBM, 64 rows of 4096, 32 / 8 heads, 118 and 117 of 80, 138
+  // and 137 of 96.
   if constexpr (sizeof(T) == 2) {
     if (dim <= 80) return launch_dim<T, 128, 80>(a, op, cache, layer, s);
     if (dim <= 96) return launch_dim<T, 128, 96>(a, op, cache, layer, s);
